@@ -448,6 +448,110 @@ int tm_residual_gate_rms_norm_modulate_int8_quant(
     const void* scale, const int64_t* index, int64_t table_stride, int64_t rows, int64_t cols,
     void* stream);
 
+/* ---- 4-bit block formats ------------------------------------------------ */
+/*
+ * A value is an e2m1 code (two to a byte, the even element in the low half)
+ * times a scale shared by a block of consecutive elements of a row:
+ *   TM_FP4_NV  blocks of 16, e4m3 scale, times an fp32 scale of the row or tensor
+ *   TM_FP4_MX  blocks of 32, e8m0 (power of two) scale
+ * Block scales are stored in tiles of 128 rows x 4 blocks (512 bytes): row r
+ * and block c of a tile at byte (r % 32) * 16 + (r / 32) * 4 + c; the tiles of
+ * 128 rows are contiguous along the row.  The quantising calls write the whole
+ * buffer, 0 where rows or blocks only pad a tile.  No reference counterpart:
+ * the reference's linears stop at 8 bits.
+ */
+#define TM_FP4_NV 0
+#define TM_FP4_MX 1
+
+/* Bytes of the block-scale buffer of a [rows, cols] tensor. */
+int tm_fp4_block_scales_size(int64_t rows, int64_t cols, int format, uint64_t* bytes);
+
+/*
+ * Quantisation to a 4-bit block format, the counterpart of
+ * tm_dynamic_scaled_int8_quant / tm_static_scaled_int8_quant (it converts
+ * weights too: a weight's rows are its output channels).
+ *   TM_FP4_NV  o = given_scale[0], or fp32(max(max_k |x[r,k]|, 2^-100) / 2688),
+ *              written to scales[r];  s = e4m3(m / (6 o)), at most 448, for the
+ *              block maximum m;  q = e2m1(x / (o s)), 0 where s = 0
+ *   TM_FP4_MX  s = 2^(floor(log2 m) - 2), at least 2^-127;  q = e2m1(x / s)
+ * Each quotient is rounded once, from its exact value, to nearest (ties to
+ * even), q to at most 6.  Exactly one of scales and given_scale is non-NULL for
+ * TM_FP4_NV, neither for TM_FP4_MX.  given_scale must be positive, from 2^-110 to 2^110.
+ * A row with an inf or a NaN gets the outer scale NaN, block scales and codes 0;
+ * where there is no outer scale to be written, such a block gets the scale NaN and
+ * codes 0: either way the products with it are NaN.
+ * input: [rows, cols] bf16 / fp16 / fp32, any alignment and row stride; rows of
+ * up to 32768 16-bit (16384 32-bit) elements on 16-byte boundaries are read
+ * once.  q: [rows, cols / 2], contiguous, 16-byte aligned.  cols % 32 == 0.
+ */
+int tm_scaled_fp4_quant(uint8_t* q, uint8_t* block_scales, float* scales, const float* given_scale,
+                        const void* input, int input_dtype, int format, int64_t rows, int64_t cols,
+                        int64_t input_row_stride, void* stream);
+
+/*
+ * The values of a 4-bit tensor: out = (q * s) * o, rounded to the output type.
+ * scales: NULL (o = 1), or 1 or `rows` fp32 values.  out [rows, cols] contiguous,
+ * 16-byte aligned.
+ */
+int tm_dequantize_fp4(void* out, int out_dtype, const uint8_t* q, const uint8_t* block_scales,
+                      const float* scales, int64_t scales_numel, int format, int64_t rows,
+                      int64_t cols, void* stream);
+
+/*
+ * The adaLN producers (tm_modulate_int8_quant, tm_rms_norm_modulate_int8_quant,
+ * tm_residual_gate_rms_norm_modulate_int8_quant: the same hidden state and
+ * residual, bit for bit) followed by tm_scaled_fp4_quant with the row's own
+ * scale (`scales`, TM_FP4_NV; NULL for TM_FP4_MX).  cols % 32 == 0, up to 32768;
+ * table_stride % 8 == 0; 16-byte aligned pointers.
+ */
+int tm_modulate_fp4_quant(uint8_t* q, uint8_t* block_scales, float* scales, void* hidden_out,
+                          const void* x, const void* shift, const void* scale, const int64_t* index,
+                          int64_t table_stride, int format, int64_t rows, int64_t cols,
+                          void* stream);
+int tm_rms_norm_modulate_fp4_quant(uint8_t* q, uint8_t* block_scales, float* scales,
+                                   void* hidden_out, const void* x, const void* norm_weight,
+                                   float eps, const void* shift, const void* scale,
+                                   const int64_t* index, int64_t table_stride, int format,
+                                   int64_t rows, int64_t cols, void* stream);
+int tm_residual_gate_rms_norm_modulate_fp4_quant(
+    uint8_t* q, uint8_t* block_scales, float* scales, void* residual_out, void* hidden_out,
+    const void* residual, const void* branch, const void* gate, const void* norm_weight, float eps,
+    const void* shift, const void* scale, const int64_t* index, int64_t table_stride, int format,
+    int64_t rows, int64_t cols, void* stream);
+
+/*
+ * Block-scaled 4-bit GEMM:
+ *   out[m,n] = act(scale_a[m] * (scale_b[n] * sum_k va[m,k] vb[n,k]) (+ bias[n]))
+ * with va = q * s, accumulated in fp32 and rounded once on output (the
+ * activation too: unlike the int8 epilogues, nothing is rounded before it).
+ * a: [m, k / 2] codes, row stride lda bytes; b: the [n, k / 2] weight codes,
+ * row stride ldb bytes (both strides multiples of 16); block scales as
+ * tm_scaled_fp4_quant writes them; scale_a / scale_b: 1 or m / n fp32 values
+ * (TM_FP4_NV), NULL (TM_FP4_MX).  bias: NULL or [n] in out_dtype (bf16 / fp16).
+ * epilogue: TM_EPI_GELU_TANH, or TM_EPI_SWIGLU (n interleaved columns in, n / 2
+ * out, n % 64 == 0).  k % 32 == 0, n % 8 == 0, ldo % 8 == 0; a, b, the block
+ * scales and out 16-byte aligned.
+ */
+int tm_scaled_mm_fp4(void* out, int out_dtype, const uint8_t* a, const uint8_t* b,
+                     const uint8_t* block_scales_a, const uint8_t* block_scales_b,
+                     const float* scale_a, int64_t scale_a_numel, const float* scale_b,
+                     int64_t scale_b_numel, const void* bias, int format, int64_t m, int64_t n,
+                     int64_t k, int64_t lda, int64_t ldb, int64_t ldo, uint32_t epilogue,
+                     void* stream);
+
+/*
+ * tm_scaled_mm_fp4 with a forced configuration, for tests and benchmarks:
+ * tile 32, 64, 128 = one CTA per 128 weight rows x that many tokens (32 and 64
+ * take m up to 32 and 64), with `splits` (1, 2, 4, 8, at most the number of
+ * 256-element k-blocks) slices of K; 1256 = the CTA-pair kernel, splits 1.
+ */
+int tm_scaled_mm_fp4_tile(void* out, int out_dtype, const uint8_t* a, const uint8_t* b,
+                          const uint8_t* block_scales_a, const uint8_t* block_scales_b,
+                          const float* scale_a, int64_t scale_a_numel, const float* scale_b,
+                          int64_t scale_b_numel, const void* bias, int format, int64_t m, int64_t n,
+                          int64_t k, int64_t lda, int64_t ldb, int64_t ldo, uint32_t epilogue,
+                          int tile, int splits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -28,7 +28,8 @@ CAPI_SO = LIB / "libtaomate_w8a8.so"
 TORCH_SO = LIB / "libtaomate_w8a8_torch.so"
 STAMP = LIB / "build.stamp"
 
-CUDA_SOURCES = ("runtime.cu", "quant.cu", "gemm_i8.cu", "peer_memory.cu", "lora_down.cu")
+CUDA_SOURCES = ("runtime.cu", "quant.cu", "gemm_i8.cu", "peer_memory.cu", "lora_down.cu",
+                "quant_fp4.cu", "gemm_fp4.cu")
 TORCH_SOURCES = ("torch_ops.cpp",)
 ARCH_FLAGS = ("-gencode", "arch=compute_100a,code=sm_100a")
 NVCC_FLAGS = (*ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-shared")
@@ -83,7 +84,8 @@ def _run(cmd: list[str], verbose: bool) -> None:
 def build_capi(verbose: bool = False) -> Path:
     LIB.mkdir(exist_ok=True)
     tmp = CAPI_SO.with_suffix(".so.tmp")
-    cmd = [_nvcc(), *NVCC_FLAGS, "-o", str(tmp), *(str(CSRC / s) for s in CUDA_SOURCES)]
+    cmd = [_nvcc(), *NVCC_FLAGS, "--threads", "0", "-o", str(tmp),
+           *(str(CSRC / s) for s in CUDA_SOURCES)]
     _run(cmd, verbose)
     os.replace(tmp, CAPI_SO)
     return CAPI_SO

@@ -29,12 +29,18 @@ TM_DTYPE_BF16 = 0
 TM_DTYPE_FP16 = 1
 TM_DTYPE_FP32 = 2
 
+TM_FP4_NV = 0
+TM_FP4_MX = 1
+
 TM_EPI_GELU_TANH = 0x1
 TM_EPI_SWIGLU = 0x2
 TM_SPLITK_NOALLOC_MAX_BYTES = 16 << 20
 
 _GEMM = [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_i64, c_void_p, c_i64, c_void_p,
          c_i64, c_i64, c_i64, c_i64, c_i64, c_i64]
+
+_GEMM_FP4 = [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_void_p,
+             c_i64, c_void_p, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_u32]
 
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tm_status_string": (c_char_p, [c_int]),
@@ -98,6 +104,25 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tm_residual_gate_rms_norm_modulate_int8_quant": (
         c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                 c_float, c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_i64, c_void_p]),
+    "tm_fp4_block_scales_size": (c_int, [c_i64, c_i64, c_int, ctypes.POINTER(ctypes.c_uint64)]),
+    "tm_scaled_fp4_quant": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_i64, c_i64,
+                c_i64, c_void_p]),
+    "tm_dequantize_fp4": (
+        c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_i64, c_int, c_i64, c_i64,
+                c_void_p]),
+    "tm_modulate_fp4_quant": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                c_i64, c_int, c_i64, c_i64, c_void_p]),
+    "tm_rms_norm_modulate_fp4_quant": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_void_p,
+                c_void_p, c_void_p, c_i64, c_int, c_i64, c_i64, c_void_p]),
+    "tm_residual_gate_rms_norm_modulate_fp4_quant": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_i64, c_int, c_i64, c_i64,
+                c_void_p]),
+    "tm_scaled_mm_fp4": (c_int, [*_GEMM_FP4, c_void_p]),
+    "tm_scaled_mm_fp4_tile": (c_int, [*_GEMM_FP4, c_int, c_int, c_void_p]),
 }
 
 

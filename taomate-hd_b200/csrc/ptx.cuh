@@ -383,6 +383,60 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar, uint16_t cta_mas
       : "memory");
 }
 
+// ---------------------------------------------------------------- block-scaled 4-bit
+// Shared-memory matrix descriptor of one 512-byte scale tile for tcgen05.cp
+// .32x128b: 32 rows of 16 bytes, no swizzle, 8-row groups 128 bytes apart.
+__device__ __forceinline__ uint64_t make_desc_scale_tile(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);  // start address
+  d |= static_cast<uint64_t>(128u >> 4) << 32;               // SBO = 128 B
+  d |= static_cast<uint64_t>(1u) << 46;                      // descriptor version (sm_100)
+  return d;
+}
+
+// Copy one scale tile to 4 TMEM columns, the 32 lanes repeated in every lane
+// quarter.  Ordered before later tcgen05.mma of the issuing thread.  In a pair
+// each CTA's tile goes to its own TMEM.
+template <bool kPair>
+__device__ __forceinline__ void tmem_copy_scale_tile(uint32_t taddr, uint64_t desc) {
+  if constexpr (kPair)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+                 : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+                 : "memory");
+}
+
+// D[tmem] (+)= (A * scale_A) (B * scale_B)^T over 64 e2m1 elements of K, fp32
+// accumulation.  kBlock 16: four e4m3 scales a row; 32: two e8m0 scales, the
+// pair of the TMEM word picked by the descriptor's scale ids.
+template <bool kPair, int kBlock>
+__device__ __forceinline__ void umma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                         uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                         uint32_t accumulate) {
+  static_assert(kBlock == 16 || kBlock == 32, "block of 16 or 32 elements");
+#define TM_UMMA_FP4(GROUP, VEC)                                                              \
+  asm volatile(                                                                              \
+      "{\n\t.reg .pred p;\n\t"                                                               \
+      "setp.ne.b32 p, %4, 0;\n\t"                                                            \
+      "tcgen05.mma.cta_group::" GROUP ".kind::mxf4nvf4.block_scale.scale_vec::" VEC          \
+      " [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d_tmem),                                \
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)              \
+      : "memory")
+  if constexpr (kPair) {
+    if constexpr (kBlock == 16)
+      TM_UMMA_FP4("2", "4X");
+    else
+      TM_UMMA_FP4("2", "2X");
+  } else {
+    if constexpr (kBlock == 16)
+      TM_UMMA_FP4("1", "4X");
+    else
+      TM_UMMA_FP4("1", "2X");
+  }
+#undef TM_UMMA_FP4
+}
+
 // Hardware tanh approximation (MUFU, max relative error about 2^-11).
 __device__ __forceinline__ float tanh_approx(float x) {
   float y;
@@ -406,6 +460,18 @@ __host__ __device__ constexpr uint32_t make_idesc_bf16(int m, int n) {
          | (1u << 10)                              // B: BF16
          | (static_cast<uint32_t>(n >> 3) << 17)
          | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// Instruction descriptor, kind::mxf4nvf4: e2m1 A and B, both K-major, fp32 D;
+// e8m0 or e4m3 scales, `sf_id` the first scale of the TMEM word to use (0 or 2).
+__host__ __device__ constexpr uint32_t make_idesc_fp4(int m, int n, bool e8m0, int sf_id) {
+  return (static_cast<uint32_t>(sf_id) << 4)       // scale id of B
+         | (1u << 7)                               // A: e2m1
+         | (1u << 10)                              // B: e2m1
+         | (static_cast<uint32_t>(n >> 3) << 17)
+         | (static_cast<uint32_t>(e8m0) << 23)     // scale type
+         | (static_cast<uint32_t>(m >> 7) << 27)
+         | (static_cast<uint32_t>(sf_id) << 29);   // scale id of A
 }
 
 }  // namespace tmw

@@ -1,0 +1,784 @@
+// Quantisation to the 4-bit block formats (fp4.cuh), its inverse, and the
+// adaLN producers fused into it.
+//
+//   TM_FP4_NV  o = fp32(max(max |x|, 2^-100) / 2688) for the row (2688 = 448 x 6, the
+//              largest e4m3 times the largest e2m1), or a given o;
+//              s = e4m3(m / (6 o)) for the block maximum m, at most 448;
+//              q = e2m1(x / (o s)), 0 where s = 0
+//   TM_FP4_MX  s = 2^(floor(log2 m) - 2), at least 2^-127;  q = e2m1(x / s)
+//
+// Every quotient is rounded once, from its exact value, to nearest with ties
+// to even.  For TM_FP4_MX that is free (s is a power of two).  For TM_FP4_NV
+// the fp32 product y = x * (1 / (o s)) is off by up to 2^-22, and bf16 data
+// meets the borders between two codes (or passes them by less than that) once
+// in some thousand elements.  So y (1 - 2^-21) and y (1 + 2^-21) are both
+// converted: where the codes agree no border lies between them and the code is
+// right; where they differ the border t decides by the sign of x - (t s) o,
+// which one fma gives exactly (t s has at most 7 bits, so the product is not
+// rounded before the subtraction).  The scale's rounding is decided the same
+// way, with its border t: m - (6 t) o.
+//
+// The kernels are bound by HBM: 2 bytes read and 0.56 written per bf16 element.
+// As in the int8 kernels a group of 32..256 threads owns a row and holds it in
+// registers between the row maximum and the conversion; a thread's unit is 16
+// elements (32 contiguous bytes of bf16), i.e. a whole TM_FP4_NV block and half
+// a TM_FP4_MX one, so the block maximum needs no shuffle or one.  Maxima are
+// taken on the bits of |x| as unsigned integers, which order NaN above inf
+// above every finite value: one reduction finds the maximum and what is not
+// finite.
+#include "fp4.cuh"
+#include "rows.cuh"
+
+namespace tmw {
+namespace {
+
+enum Fp4Kind : int {
+  kNvDynamic = 0,  // row scale from the row's maximum
+  kNvGiven = 1,    // one given scale
+  kMx = 2
+};
+
+struct Fp4Params : QuantParams {
+  uint8_t* codes;       // [rows, cols / 2]
+  uint8_t* blocks;      // tiles
+  int64_t ktiles;       // tiles along a row
+  int64_t padded_rows;  // rows, rounded up to whole tiles
+};
+
+constexpr uint32_t kInfBits = 0x7f800000u;
+
+// Eight values -> eight e2m1 codes, v[0] in the low half of the first byte;
+// to nearest, ties to even, at most 6.
+__device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+
+// Two values -> two e4m3 bytes, `lo` in the low one; at most 448.
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+__device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t pair) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(pair)));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// Value of an e2m1 magnitude code 0..7.
+__device__ __forceinline__ float e2m1_value(uint32_t c) {
+  // codes 2..7 have the bits of an fp32 number's low exponent and top mantissa
+  return c < 2 ? 0.5f * static_cast<float>(c)
+               : __uint_as_float(((c >> 1) + 126u) << 23 | (c & 1u) << 22);
+}
+
+__device__ __forceinline__ float rcp_approx(float v) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+constexpr float kBelow = 1.0f - 4.76837158203125e-07f;  // 1 - 2^-21
+constexpr float kAbove = 1.0f + 4.76837158203125e-07f;
+
+// e4m3 scale byte of a block with maximum m under the outer scale o;
+// inv6o is 1 / (6 o) to 2^-22.
+__device__ __forceinline__ uint32_t nv_scale_byte(float m, float o, float inv6o) {
+  const float z = __fmul_rn(m, inv6o);
+  const uint32_t pair = e4m3x2(__fmul_rn(z, kBelow), __fmul_rn(z, kAbove));
+  const uint32_t lo = pair & 0xffu, hi = pair >> 8;
+  if (lo == hi) return lo;
+  const float2 v = e4m3x2_to_f32(pair);
+  const float d = __fmaf_rn(-3.0f * (v.x + v.y), o, m);  // m - 6 (lo + hi) / 2 o, exact sign
+  return d > 0.0f || (d == 0.0f && (lo & 1u)) ? hi : lo;
+}
+
+// Resolve the codes of eight values that lie within 2^-21 of a border: lo and
+// hi are the conversions from just below and just above.
+__device__ __forceinline__ uint32_t resolve8(uint32_t lo, uint32_t hi, const float (&x)[8], float s,
+                                             float o) {
+  uint32_t out = lo;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t a = (lo >> (4 * j)) & 7u, b = (hi >> (4 * j)) & 7u;
+    if (a != b) {
+      const float ts = __fmul_rn(0.5f * (e2m1_value(a) + e2m1_value(b)), s);
+      const float d = __fmaf_rn(-ts, o, fabsf(x[j]));
+      if (d > 0.0f || (d == 0.0f && (a & 1u)))
+        out = (out & ~(7u << (4 * j))) | (b << (4 * j));
+    }
+  }
+  return out;
+}
+
+// Eight codes of x under block scale s and outer scale o; inv = 1 / (o s).
+__device__ __forceinline__ uint32_t nv_codes8(const float (&x)[8], float inv, float s, float o) {
+  const float below = __fmul_rn(inv, kBelow), above = __fmul_rn(inv, kAbove);
+  float a[8], b[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    a[j] = __fmul_rn(x[j], below);
+    b[j] = __fmul_rn(x[j], above);
+  }
+  const uint32_t lo = e2m1x8(a), hi = e2m1x8(b);
+  return lo == hi ? lo : resolve8(lo, hi, x, s, o);
+}
+
+__device__ __forceinline__ uint32_t mx_codes8(const float (&x)[8], float inv) {
+  float a[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a[j] = __fmul_rn(x[j], inv);  // exact, or far below the first border
+  return e2m1x8(a);
+}
+
+// ---- a thread's 16 elements ----
+template <typename T>
+struct Unit {  // 16-bit types: 16 values in 32 bytes
+  uint4 raw[2];
+};
+template <>
+struct Unit<float> {
+  uint4 raw[4];
+};
+
+// 32 bytes; `wide`: the address is a multiple of 32 (one load), else of 16.
+__device__ __forceinline__ void ld_stream32(const void* p, bool wide, uint4& a, uint4& b) {
+  if (wide) {
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z),
+                   "=r"(b.w)
+                 : "l"(p));
+  } else {
+    a = ld_cached16(p);
+    b = ld_cached16(static_cast<const uint8_t*>(p) + 16);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_unit(Unit<T>& u, const T* p, bool wide) {
+#pragma unroll
+  for (int h = 0; h < static_cast<int>(sizeof(T)) / 2; ++h)
+    ld_stream32(reinterpret_cast<const uint8_t*>(p) + 32 * h, wide, u.raw[2 * h], u.raw[2 * h + 1]);
+}
+
+template <typename T>
+__device__ __forceinline__ void clear_unit(Unit<T>& u) {
+#pragma unroll
+  for (int h = 0; h < static_cast<int>(sizeof(T)); ++h) u.raw[h] = make_uint4(0u, 0u, 0u, 0u);
+}
+
+// Element by element: any alignment (16 elements from p).
+template <typename T>
+__device__ __forceinline__ void load_unit_scalar(Unit<T>& u, const T* p) {
+  T* e = reinterpret_cast<T*>(u.raw);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) e[j] = p[j];
+}
+
+// Largest |x| of the unit as the bits of an fp32 number (NaN > inf > finite).
+template <typename T>
+__device__ __forceinline__ uint32_t unit_max_bits(const Unit<T>& u) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(u.raw);
+  if constexpr (sizeof(T) == 2) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = __vmaxu2(m, w[j] & 0x7fff7fffu);
+    const uint16_t top = static_cast<uint16_t>(max(m & 0xffffu, m >> 16));
+    return __float_as_uint(to_f32<T>(*reinterpret_cast<const T*>(&top))) & 0x7fffffffu;
+  } else {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) m = max(m, w[j] & 0x7fffffffu);
+    return m;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void unit_values(const Unit<T>& u, int half, float (&v)[8]) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&u.raw[half]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = __uint_as_float(w[j] << 16);
+      v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    }
+  } else {
+    const T* e = reinterpret_cast<const T*>(u.raw) + 8 * half;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(e[j]);
+  }
+}
+
+// Largest of one value per thread over the row's group; every thread of the
+// block takes part.
+__device__ __forceinline__ uint32_t group_max_bits(uint32_t v, int tpr, uint32_t* red) {
+  v = __reduce_max_sync(0xffffffffu, v);  // a group is whole warps
+  if (tpr > 32) {
+    const int warp = threadIdx.x >> 5;
+    const int wpr = tpr >> 5;
+    const int first = warp / wpr * wpr;
+    __syncthreads();  // `red` may still be read from its previous use
+    if ((threadIdx.x & 31) == 0) red[warp] = v;
+    __syncthreads();
+    v = red[first];
+    for (int w = 1; w < wpr; ++w) v = max(v, red[first + w]);
+  }
+  return v;
+}
+
+// What a row's conversion needs.
+struct RowScale {
+  float o;      // outer scale (TM_FP4_NV)
+  float inv6o;  // 1 / (6 o) to 2^-22
+  bool bad;     // the row holds an inf or a NaN (its own scale is NaN, blocks and codes 0)
+};
+
+__device__ __forceinline__ RowScale row_scale(uint32_t max_bits) {
+  RowScale r;
+  r.bad = max_bits >= kInfBits;
+  const float a = fmaxf(__uint_as_float(max_bits), 7.888609052210118e-31f);  // 2^-100
+  r.o = r.bad ? __int_as_float(0x7fffffff) : __fdiv_rn(a, 2688.0f);
+  r.inv6o = rcp_approx(__fmul_rn(6.0f, r.o));
+  return r;
+}
+
+__device__ __forceinline__ RowScale given_scale(float o) {
+  return RowScale{o, rcp_approx(__fmul_rn(6.0f, o)), false};
+}
+
+// Convert one unit (16 elements, block maximum `m_bits` as fp32 bits) and
+// return its scale byte; codes to c[0..1].
+template <typename T, int KIND>
+__device__ __forceinline__ uint32_t convert_unit(const Unit<T>& u, uint32_t m_bits,
+                                                 const RowScale& rs, uint32_t (&c)[2]) {
+  c[0] = c[1] = 0u;
+  float v[8];
+  if constexpr (KIND == kMx) {
+    if (m_bits >= kInfBits) return 0xffu;  // e8m0 NaN
+    const int e = static_cast<int>(m_bits >> 23) - 2;  // an fp32 subnormal maximum: 2^-127
+    const uint32_t byte = static_cast<uint32_t>(max(e, 0));
+    // 2^(127 - byte); byte <= 252, so the factor is a normal number
+    const float inv = __uint_as_float((254u - byte) << 23);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      unit_values(u, h, v);
+      c[h] = mx_codes8(v, inv);
+    }
+    return byte;
+  } else {
+    if (KIND == kNvGiven && m_bits >= kInfBits) return 0x7fu;  // e4m3 NaN
+    if (rs.bad) return 0u;
+    const uint32_t byte = nv_scale_byte(__uint_as_float(m_bits), rs.o, rs.inv6o);
+    if (byte == 0u) return 0u;
+    const float s = e4m3x2_to_f32(byte).x;
+    const float inv = rcp_approx(__fmul_rn(rs.o, s));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      unit_values(u, h, v);
+      c[h] = nv_codes8(v, inv, s, rs.o);
+    }
+    return byte;
+  }
+}
+
+// Store the codes and the scale byte of unit `unit` of `row`.  TM_FP4_MX blocks
+// span two units (adjacent lanes); the even one stores the byte.
+template <int KIND>
+__device__ __forceinline__ void store_unit(const Fp4Params& p, int64_t row, int64_t unit,
+                                           const uint32_t (&c)[2], uint32_t byte) {
+  *reinterpret_cast<uint2*>(p.codes + row * (p.cols / 2) + unit * 8) = make_uint2(c[0], c[1]);
+  if (KIND != kMx || (unit & 1) == 0)
+    p.blocks[fp4_scale_offset(row, KIND == kMx ? unit >> 1 : unit, p.ktiles)] =
+        static_cast<uint8_t>(byte);
+}
+
+// Zero scale byte of a unit that only pads a tile.
+template <int KIND>
+__device__ __forceinline__ void store_pad(const Fp4Params& p, int64_t row, int64_t unit) {
+  if (KIND != kMx || (unit & 1) == 0)
+    p.blocks[fp4_scale_offset(row, KIND == kMx ? unit >> 1 : unit, p.ktiles)] = 0;
+}
+
+// A row group per row, the row in registers.  MODE: an adaLN producer, or
+// kDynamic for a plain row.
+template <typename T, int VPT, int MODE, int KIND>
+__global__ void __launch_bounds__(256) quant_fp4_rows_kernel(const Fp4Params p, const bool wide) {
+  griddep_wait();  // the rows may come from the previous kernel on the stream
+  griddep_launch_dependents();
+  __shared__ double red_f64[8];
+  uint32_t* red = reinterpret_cast<uint32_t*>(red_f64);
+  const int tpr = 1 << p.tpr_log2;
+  const int t = threadIdx.x & (tpr - 1);
+  const int64_t row =
+      static_cast<int64_t>(blockIdx.x) * (blockDim.x >> p.tpr_log2) + (threadIdx.x >> p.tpr_log2);
+  const bool active = row < p.rows;
+  const int64_t units = p.cols / 16;
+  const int64_t pad_units = p.ktiles * (KIND == kMx ? 8 : 4);
+  const T* xr = static_cast<const T*>(p.x) + (active ? row : 0) * p.ldx;
+  constexpr bool kAdaLN = MODE != kDynamic;
+
+  Unit<T> u[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int64_t unit = t + static_cast<int64_t>(i) * tpr;
+    if (active && unit < units)
+      load_unit(u[i], xr + unit * 16, wide);
+    else
+      clear_unit(u[i]);
+  }
+  if constexpr (kAdaLN) {
+    static_assert(std::is_same<T, __nv_bfloat16>::value, "adaLN modes are bf16");
+    uint4 raw[2 * VPT], pre_sc[2 * VPT], pre_sh[2 * VPT];
+#pragma unroll
+    for (int i = 0; i < 2 * VPT; ++i) raw[i] = u[i >> 1].raw[i & 1];
+    if constexpr (MODE == kModulateRows) {
+      const int64_t trow = active ? row : 0;
+#pragma unroll
+      for (int i = 0; i < 2 * VPT; ++i) {
+        const int64_t vi = vec_index<true>(t, i, tpr);
+        const bool in = active && vi < 2 * units;
+        const __nv_bfloat16* sc = p.mod_scale + trow * p.table_stride + vi * 8;
+        const __nv_bfloat16* sh = p.shift + trow * p.table_stride + vi * 8;
+        pre_sc[i] = in ? ld_cached16(sc) : make_uint4(0u, 0u, 0u, 0u);
+        pre_sh[i] = in ? ld_cached16(sh) : make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+    adaln_rows<2 * VPT, MODE, true>(p, raw, pre_sc, pre_sh, row, t, tpr, 2 * units, active,
+                                    red_f64);
+#pragma unroll
+    for (int i = 0; i < 2 * VPT; ++i) u[i >> 1].raw[i & 1] = raw[i];
+  }
+
+  uint32_t m[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    m[i] = unit_max_bits(u[i]);
+    if constexpr (KIND == kMx) m[i] = max(m[i], __shfl_xor_sync(0xffffffffu, m[i], 1));
+  }
+  RowScale rs{};
+  if constexpr (KIND == kNvDynamic) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) top = max(top, m[i]);
+    rs = row_scale(group_max_bits(top, tpr, red));
+    if (active && t == 0) p.scales[row] = rs.o;
+  } else if constexpr (KIND == kNvGiven) {
+    rs = given_scale(__ldg(p.static_scale));
+  }
+  if (row >= p.padded_rows) return;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int64_t unit = t + static_cast<int64_t>(i) * tpr;
+    if (active && unit < units) {
+      uint32_t c[2];
+      const uint32_t byte = convert_unit<T, KIND>(u[i], m[i], rs, c);
+      store_unit<KIND>(p, row, unit, c, byte);
+    } else if (unit < pad_units) {
+      store_pad<KIND>(p, row, unit);
+    }
+  }
+}
+
+// Rows of any width and alignment: a block per row, the row read twice (once
+// where no row maximum is needed), element by element.
+template <typename T, int KIND>
+__global__ void __launch_bounds__(256) quant_fp4_any_kernel(const Fp4Params p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  __shared__ uint32_t red[8];
+  const int64_t row = blockIdx.x;
+  const bool active = row < p.rows;
+  const int64_t units = p.cols / 16;
+  const int64_t pad_units = p.ktiles * (KIND == kMx ? 8 : 4);
+  const T* xr = static_cast<const T*>(p.x) + (active ? row : 0) * p.ldx;
+  RowScale rs{};
+  if constexpr (KIND == kNvDynamic) {
+    uint32_t top = 0;
+    if (active) {
+      for (int64_t unit = threadIdx.x; unit < units; unit += blockDim.x) {
+        Unit<T> u;
+        load_unit_scalar(u, xr + unit * 16);
+        top = max(top, unit_max_bits(u));
+      }
+    }
+    rs = row_scale(group_max_bits(top, 256, red));
+    if (active && threadIdx.x == 0) p.scales[row] = rs.o;
+  } else if constexpr (KIND == kNvGiven) {
+    rs = given_scale(__ldg(p.static_scale));
+  }
+  const int64_t lane_units = (pad_units + 255) / 256 * 256;  // whole warps: shuffles below
+  for (int64_t unit = threadIdx.x; unit < lane_units; unit += blockDim.x) {
+    Unit<T> u;
+    const bool in = active && unit < units;
+    if (in)
+      load_unit_scalar(u, xr + unit * 16);
+    else
+      clear_unit(u);
+    uint32_t m = unit_max_bits(u);
+    if constexpr (KIND == kMx) m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    if (in) {
+      uint32_t c[2];
+      const uint32_t byte = convert_unit<T, KIND>(u, m, rs, c);
+      store_unit<KIND>(p, row, unit, c, byte);
+    } else if (unit < pad_units) {
+      store_pad<KIND>(p, row, unit);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ inverse
+struct DequantParams {
+  void* out;  // [rows, cols]
+  const uint8_t* codes;
+  const uint8_t* blocks;
+  const float* scales;  // NULL: 1
+  bool per_row;
+  int64_t rows, cols, ktiles;
+  int tpr_log2;
+};
+
+// Two e2m1 codes -> two values.
+__device__ __forceinline__ float2 e2m1x2_to_f32(uint32_t byte) {
+  uint32_t h;
+  asm("{\n\t.reg .b8 b, z;\n\t"
+      "mov.b16 {b, z}, %1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b;\n\t}"
+      : "=r"(h)
+      : "h"(static_cast<uint16_t>(byte)));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+template <typename T>
+__device__ __forceinline__ void store16(T* out, const float (&v)[16]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 16; j += 4)
+      *reinterpret_cast<float4*>(out + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+  } else {
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+      } else {
+        const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+        w[j] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    reinterpret_cast<uint4*>(out)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(out)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+
+// value = (q * s) * o: q * s is exact in fp32, the product with o is rounded,
+// and the result is rounded once more to a 16-bit output type.
+template <typename T, int FORMAT>
+__global__ void __launch_bounds__(256) dequant_fp4_kernel(const DequantParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const int tpr = 1 << p.tpr_log2;
+  const int t = threadIdx.x & (tpr - 1);
+  const int64_t row =
+      static_cast<int64_t>(blockIdx.x) * (blockDim.x >> p.tpr_log2) + (threadIdx.x >> p.tpr_log2);
+  if (row >= p.rows) return;
+  const int64_t units = p.cols / 16;
+  const float o = p.scales == nullptr ? 1.0f : __ldg(p.scales + (p.per_row ? row : 0));
+  T* out = static_cast<T*>(p.out) + row * p.cols;
+#pragma unroll 4
+  for (int64_t unit = t; unit < units; unit += tpr) {
+    const uint2 c = __ldg(reinterpret_cast<const uint2*>(p.codes + row * (p.cols / 2)) + unit);
+    const uint32_t byte =
+        __ldg(p.blocks + fp4_scale_offset(row, FORMAT == TM_FP4_MX ? unit >> 1 : unit, p.ktiles));
+    float s;
+    if constexpr (FORMAT == TM_FP4_MX)  // 2^(byte - 127); 0 is the subnormal 2^-127, 255 NaN
+      s = __uint_as_float(byte == 255u ? 0x7fffffffu : byte == 0u ? 0x00400000u : byte << 23);
+    else
+      s = e4m3x2_to_f32(byte).x;
+    float v[16];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 q = e2m1x2_to_f32(((j < 4 ? c.x : c.y) >> (8 * (j & 3))) & 0xffu);
+      v[2 * j] = __fmul_rn(__fmul_rn(q.x, s), o);
+      v[2 * j + 1] = __fmul_rn(__fmul_rn(q.y, s), o);
+    }
+    store16(out + unit * 16, v);
+  }
+}
+
+// ------------------------------------------------------------------ host
+template <typename T>
+constexpr int max_units() {  // 16-element units a thread may hold in registers
+  return sizeof(T) == 2 ? 8 : 4;
+}
+
+// Threads per row (32..256) and units per thread; false: the row does not fit.
+// At most 4 units a thread while the group can still grow: 20480 x 3072 then
+// runs on 64 threads a row.
+template <typename T>
+bool pick_fp4_layout(int64_t units, int* tpr_log2, int* vpt) {
+  for (int l = 5; l <= 8; ++l) {
+    const int64_t v = (units + (1 << l) - 1) >> l;
+    if (v <= 4 || (l == 8 && v <= max_units<T>())) {
+      *tpr_log2 = l;
+      *vpt = static_cast<int>(v);
+      return true;
+    }
+  }
+  return false;
+}
+
+template <typename T, int MODE, int KIND>
+int launch_rows(Fp4Params p, int tpr_log2, int vpt, bool wide, cudaStream_t stream) {
+  p.tpr_log2 = tpr_log2;
+  const int rpb = 256 >> tpr_log2;
+  const int64_t grid = (p.padded_rows + rpb - 1) / rpb;
+  if (grid > 0x7fffffffLL) return TM_ERR_TOO_LARGE;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaError_t err = cudaErrorInvalidValue;
+  const auto go = [&](auto tag) {
+    err = launch_with_pdl(cfg, nullptr, 0, quant_fp4_rows_kernel<T, decltype(tag)::value, MODE, KIND>,
+                          p, wide);
+  };
+  if (vpt <= 1) go(std::integral_constant<int, 1>{});
+  else if (vpt <= 2) go(std::integral_constant<int, 2>{});
+  else if (vpt <= 3) go(std::integral_constant<int, 3>{});
+  else if (vpt <= 4) go(std::integral_constant<int, 4>{});
+  else if constexpr (max_units<T>() > 4) {
+    if (vpt <= 6) go(std::integral_constant<int, 6>{});
+    else if (vpt <= 8) go(std::integral_constant<int, 8>{});
+    else return TM_ERR_UNSUPPORTED;
+  } else {
+    return TM_ERR_UNSUPPORTED;
+  }
+  return err == cudaSuccess ? check_launch() : TM_ERR_CUDA;
+}
+
+inline bool multiple_of(const void* ptr, int64_t stride_bytes, int64_t n) {
+  return reinterpret_cast<uintptr_t>(ptr) % n == 0 && stride_bytes % n == 0;
+}
+
+template <typename T, int KIND>
+int launch_plain(const Fp4Params& p, cudaStream_t stream) {
+  int tpr_log2 = 0, vpt = 0;
+  const int64_t stride = p.ldx * static_cast<int64_t>(sizeof(T));
+  if (multiple_of(p.x, stride, 16) && pick_fp4_layout<T>(p.cols / 16, &tpr_log2, &vpt))
+    return launch_rows<T, kDynamic, KIND>(p, tpr_log2, vpt, multiple_of(p.x, stride, 32), stream);
+  if (p.padded_rows > 0x7fffffffLL) return TM_ERR_TOO_LARGE;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.padded_rows));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  if (launch_with_pdl(cfg, nullptr, 0, quant_fp4_any_kernel<T, KIND>, p) != cudaSuccess)
+    return TM_ERR_CUDA;
+  return check_launch();
+}
+
+template <int KIND>
+int launch_typed(const Fp4Params& p, int dtype, cudaStream_t stream) {
+  switch (dtype) {
+    case TM_DTYPE_BF16: return launch_plain<__nv_bfloat16, KIND>(p, stream);
+    case TM_DTYPE_FP16: return launch_plain<__half, KIND>(p, stream);
+    case TM_DTYPE_FP32: return launch_plain<float, KIND>(p, stream);
+    default: return TM_ERR_DTYPE;
+  }
+}
+
+// Shape checks of every quantising entry point, and the stored form's geometry.
+int set_geometry(Fp4Params& p, int format, int64_t rows, int64_t cols, int64_t ld) {
+  if (format != TM_FP4_NV && format != TM_FP4_MX) return TM_ERR_UNSUPPORTED;
+  if (rows < 0 || cols <= 0 || cols % 32 != 0 || ld < cols) return TM_ERR_SHAPE;
+  p.rows = rows;
+  p.cols = cols;
+  p.ldx = ld;
+  p.padded_rows = round_up(rows, 128);
+  p.ktiles = round_up(cols / fp4_block(format), 4) / 4;
+  return TM_OK;
+}
+
+template <int MODE>
+int launch_adaln(Fp4Params p, int format, cudaStream_t stream) {
+  if (p.table_stride % 8 != 0 || !aligned16(p.x) || !aligned16(p.shift) ||
+      !aligned16(p.mod_scale) || (p.hidden_out != nullptr && !aligned16(p.hidden_out)) ||
+      (!modulate_only(MODE) && !aligned16(p.norm_w)) ||
+      (MODE == kResGateRmsModulate &&
+       (!aligned16(p.branch) || !aligned16(p.gate) || !aligned16(p.residual_out))))
+    return TM_ERR_ALIGNMENT;
+  // as for the int8 producers: one warp a row in the RMSNorm modes while the
+  // row fits (widths up to 3072)
+  int tpr_log2 = 5, vpt = 0;
+  const int64_t units = p.cols / 16;
+  if (!modulate_only(MODE) && units <= 32 * 6)
+    vpt = static_cast<int>((units + 31) / 32);
+  else if (!pick_fp4_layout<__nv_bfloat16>(units, &tpr_log2, &vpt))
+    return TM_ERR_TOO_LARGE;
+  const bool wide = multiple_of(p.x, p.ldx * 2, 32);
+  return format == TM_FP4_MX
+             ? launch_rows<__nv_bfloat16, MODE, kMx>(p, tpr_log2, vpt, wide, stream)
+             : launch_rows<__nv_bfloat16, MODE, kNvDynamic>(p, tpr_log2, vpt, wide, stream);
+}
+
+template <typename T>
+int launch_dequant(const DequantParams& p, int format, cudaStream_t stream) {
+  const int rpb = 256 >> p.tpr_log2;
+  const int64_t grid = (p.rows + rpb - 1) / rpb;
+  if (grid > 0x7fffffffLL) return TM_ERR_TOO_LARGE;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  const cudaError_t err =
+      format == TM_FP4_MX ? launch_with_pdl(cfg, nullptr, 0, dequant_fp4_kernel<T, TM_FP4_MX>, p)
+                          : launch_with_pdl(cfg, nullptr, 0, dequant_fp4_kernel<T, TM_FP4_NV>, p);
+  return err == cudaSuccess ? check_launch() : TM_ERR_CUDA;
+}
+
+// The adaLN arguments common to the producers.
+int adaln_params(Fp4Params& p, uint8_t* q, uint8_t* block_scales, float* scales, void* hidden_out,
+                 const void* x, const void* shift, const void* scale, const int64_t* index,
+                 int64_t table_stride, int format, int64_t rows, int64_t cols) {
+  if (int s = set_geometry(p, format, rows, cols, cols)) return s;
+  if (table_stride < cols) return TM_ERR_SHAPE;
+  if (rows == 0) return TM_OK;
+  if (!q || !block_scales || !x || !shift || !scale || (format == TM_FP4_NV && !scales))
+    return TM_ERR_NULL_POINTER;
+  if (!aligned16(q)) return TM_ERR_ALIGNMENT;
+  p.x = x;
+  p.codes = q;
+  p.blocks = block_scales;
+  p.scales = scales;
+  p.hidden_out = static_cast<__nv_bfloat16*>(hidden_out);
+  p.shift = static_cast<const __nv_bfloat16*>(shift);
+  p.mod_scale = static_cast<const __nv_bfloat16*>(scale);
+  p.index = index;
+  p.table_stride = table_stride;
+  return TM_OK;
+}
+
+}  // namespace
+}  // namespace tmw
+
+extern "C" {
+
+int tm_fp4_block_scales_size(int64_t rows, int64_t cols, int format, uint64_t* bytes) {
+  if (!bytes) return TM_ERR_NULL_POINTER;
+  tmw::Fp4Params p{};
+  if (int s = tmw::set_geometry(p, format, rows, cols, cols)) return s;
+  *bytes = static_cast<uint64_t>(p.padded_rows) * static_cast<uint64_t>(p.ktiles) * 4u;
+  return TM_OK;
+}
+
+int tm_scaled_fp4_quant(uint8_t* q, uint8_t* block_scales, float* scales, const float* given_scale,
+                        const void* input, int input_dtype, int format, int64_t rows, int64_t cols,
+                        int64_t input_row_stride, void* stream) {
+  tmw::Fp4Params p{};
+  if (int s = tmw::set_geometry(p, format, rows, cols, input_row_stride)) return s;
+  if (format == TM_FP4_MX && (given_scale || scales)) return TM_ERR_UNSUPPORTED;
+  if (rows == 0) return TM_OK;
+  if (!q || !block_scales || !input || (format == TM_FP4_NV && !scales == !given_scale))
+    return TM_ERR_NULL_POINTER;  // TM_FP4_NV: one of the two scales
+  if (!tmw::aligned16(q)) return TM_ERR_ALIGNMENT;
+  p.x = input;
+  p.codes = q;
+  p.blocks = block_scales;
+  p.scales = scales;
+  p.static_scale = given_scale;
+  const cudaStream_t st = tmw::as_stream(stream);
+  if (format == TM_FP4_MX) return tmw::launch_typed<tmw::kMx>(p, input_dtype, st);
+  return given_scale ? tmw::launch_typed<tmw::kNvGiven>(p, input_dtype, st)
+                     : tmw::launch_typed<tmw::kNvDynamic>(p, input_dtype, st);
+}
+
+int tm_dequantize_fp4(void* out, int out_dtype, const uint8_t* q, const uint8_t* block_scales,
+                      const float* scales, int64_t scales_numel, int format, int64_t rows,
+                      int64_t cols, void* stream) {
+  tmw::Fp4Params g{};
+  if (int s = tmw::set_geometry(g, format, rows, cols, cols)) return s;
+  if (scales && scales_numel != 1 && scales_numel != rows) return TM_ERR_SHAPE;
+  if (rows == 0) return TM_OK;
+  if (!out || !q || !block_scales) return TM_ERR_NULL_POINTER;
+  if (!tmw::aligned16(out) || !tmw::aligned16(q)) return TM_ERR_ALIGNMENT;
+  tmw::DequantParams p{};
+  p.out = out;
+  p.codes = q;
+  p.blocks = block_scales;
+  p.scales = scales;
+  p.per_row = scales_numel == rows;
+  p.rows = rows;
+  p.cols = cols;
+  p.ktiles = g.ktiles;
+  p.tpr_log2 = 5;
+  while (p.tpr_log2 < 8 && (cols / 16) > (4ll << p.tpr_log2)) ++p.tpr_log2;
+  const cudaStream_t st = tmw::as_stream(stream);
+  switch (out_dtype) {
+    case TM_DTYPE_BF16: return tmw::launch_dequant<__nv_bfloat16>(p, format, st);
+    case TM_DTYPE_FP16: return tmw::launch_dequant<__half>(p, format, st);
+    case TM_DTYPE_FP32: return tmw::launch_dequant<float>(p, format, st);
+    default: return TM_ERR_DTYPE;
+  }
+}
+
+int tm_modulate_fp4_quant(uint8_t* q, uint8_t* block_scales, float* scales, void* hidden_out,
+                          const void* x, const void* shift, const void* scale, const int64_t* index,
+                          int64_t table_stride, int format, int64_t rows, int64_t cols,
+                          void* stream) {
+  tmw::Fp4Params p{};
+  if (int s = tmw::adaln_params(p, q, block_scales, scales, hidden_out, x, shift, scale, index,
+                                table_stride, format, rows, cols))
+    return s;
+  if (rows == 0) return TM_OK;
+  const cudaStream_t st = tmw::as_stream(stream);
+  return index == nullptr ? tmw::launch_adaln<tmw::kModulateRows>(p, format, st)
+                          : tmw::launch_adaln<tmw::kModulate>(p, format, st);
+}
+
+int tm_rms_norm_modulate_fp4_quant(uint8_t* q, uint8_t* block_scales, float* scales,
+                                   void* hidden_out, const void* x, const void* norm_weight,
+                                   float eps, const void* shift, const void* scale,
+                                   const int64_t* index, int64_t table_stride, int format,
+                                   int64_t rows, int64_t cols, void* stream) {
+  tmw::Fp4Params p{};
+  if (int s = tmw::adaln_params(p, q, block_scales, scales, hidden_out, x, shift, scale, index,
+                                table_stride, format, rows, cols))
+    return s;
+  if (rows == 0) return TM_OK;
+  if (!norm_weight) return TM_ERR_NULL_POINTER;
+  p.norm_w = static_cast<const __nv_bfloat16*>(norm_weight);
+  p.eps = eps;
+  p.inv_cols = 1.0 / static_cast<double>(cols);
+  return tmw::launch_adaln<tmw::kRmsModulate>(p, format, tmw::as_stream(stream));
+}
+
+int tm_residual_gate_rms_norm_modulate_fp4_quant(
+    uint8_t* q, uint8_t* block_scales, float* scales, void* residual_out, void* hidden_out,
+    const void* residual, const void* branch, const void* gate, const void* norm_weight, float eps,
+    const void* shift, const void* scale, const int64_t* index, int64_t table_stride, int format,
+    int64_t rows, int64_t cols, void* stream) {
+  tmw::Fp4Params p{};
+  if (int s = tmw::adaln_params(p, q, block_scales, scales, hidden_out, residual, shift, scale,
+                                index, table_stride, format, rows, cols))
+    return s;
+  if (rows == 0) return TM_OK;
+  if (!residual_out || !branch || !gate || !norm_weight) return TM_ERR_NULL_POINTER;
+  p.norm_w = static_cast<const __nv_bfloat16*>(norm_weight);
+  p.eps = eps;
+  p.inv_cols = 1.0 / static_cast<double>(cols);
+  p.branch = static_cast<const __nv_bfloat16*>(branch);
+  p.gate = static_cast<const __nv_bfloat16*>(gate);
+  p.residual_out = static_cast<__nv_bfloat16*>(residual_out);
+  return tmw::launch_adaln<tmw::kResGateRmsModulate>(p, format, tmw::as_stream(stream));
+}
+
+}  // extern "C"

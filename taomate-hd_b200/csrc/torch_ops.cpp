@@ -367,24 +367,17 @@ struct ModulateArgs {
   void* hidden;
 };
 
-ModulateArgs check_modulate(at::Tensor& out, at::Tensor& scales,
-                            const std::optional<at::Tensor>& hidden_out, const at::Tensor& x,
-                            const at::Tensor& shift, const at::Tensor& scale,
-                            const std::optional<at::Tensor>& index) {
+ModulateArgs check_modulate_inputs(const std::optional<at::Tensor>& hidden_out,
+                                   const at::Tensor& x, const at::Tensor& shift,
+                                   const at::Tensor& scale,
+                                   const std::optional<at::Tensor>& index) {
   check_cuda(x, x, "x");
-  check_cuda(out, x, "out");
-  check_cuda(scales, x, "scales");
   check_cuda(shift, x, "shift");
   check_cuda(scale, x, "scale");
   TORCH_CHECK(x.scalar_type() == at::kBFloat16 && x.is_contiguous(), "x must be contiguous bfloat16");
   ModulateArgs r{};
   r.cols = x.size(-1);
   r.rows = r.cols == 0 ? 0 : x.numel() / r.cols;
-  TORCH_CHECK(out.scalar_type() == at::kChar && out.is_contiguous() && out.numel() == x.numel(),
-              "out must be contiguous int8 with x's shape");
-  TORCH_CHECK(scales.scalar_type() == at::kFloat && scales.is_contiguous() &&
-                  scales.numel() == r.rows,
-              "scales must be contiguous float32 [rows]");
   TORCH_CHECK(shift.scalar_type() == at::kBFloat16 && scale.scalar_type() == at::kBFloat16,
               "shift/scale must be bfloat16");
   TORCH_CHECK(shift.dim() == 2 && scale.dim() == 2 && shift.sizes() == scale.sizes(),
@@ -412,6 +405,47 @@ ModulateArgs check_modulate(at::Tensor& out, at::Tensor& scales,
   return r;
 }
 
+// The int8 producers: their outputs, then the common inputs.
+ModulateArgs check_modulate(at::Tensor& out, at::Tensor& scales,
+                            const std::optional<at::Tensor>& hidden_out, const at::Tensor& x,
+                            const at::Tensor& shift, const at::Tensor& scale,
+                            const std::optional<at::Tensor>& index) {
+  check_cuda(x, x, "x");
+  check_cuda(out, x, "out");
+  check_cuda(scales, x, "scales");
+  const ModulateArgs r = check_modulate_inputs(hidden_out, x, shift, scale, index);
+  TORCH_CHECK(out.scalar_type() == at::kChar && out.is_contiguous() && out.numel() == x.numel(),
+              "out must be contiguous int8 with x's shape");
+  TORCH_CHECK(scales.scalar_type() == at::kFloat && scales.is_contiguous() &&
+                  scales.numel() == r.rows,
+              "scales must be contiguous float32 [rows]");
+  return r;
+}
+
+void check_norm_weight(const at::Tensor& weight, const at::Tensor& x, int64_t cols) {
+  check_cuda(weight, x, "weight");
+  TORCH_CHECK(weight.scalar_type() == at::kBFloat16 && weight.is_contiguous() &&
+                  weight.numel() == cols,
+              "norm weight must be contiguous bfloat16 [cols]");
+}
+
+void check_residual_gate(const at::Tensor& residual_out, const at::Tensor& residual,
+                         const at::Tensor& branch, const at::Tensor& gate,
+                         const at::Tensor& shift) {
+  check_cuda(branch, residual, "branch");
+  check_cuda(gate, residual, "gate");
+  check_cuda(residual_out, residual, "residual_out");
+  TORCH_CHECK(branch.scalar_type() == at::kBFloat16 && branch.is_contiguous() &&
+                  branch.sizes() == residual.sizes(),
+              "branch must be contiguous bfloat16 with the residual's shape");
+  TORCH_CHECK(residual_out.scalar_type() == at::kBFloat16 && residual_out.is_contiguous() &&
+                  residual_out.numel() == residual.numel(),
+              "residual_out must be contiguous bfloat16 with the residual's shape");
+  TORCH_CHECK(gate.scalar_type() == at::kBFloat16 && gate.sizes() == shift.sizes() &&
+                  gate.stride(1) == 1 && gate.stride(0) == shift.stride(0),
+              "gate must be a bfloat16 table shaped and strided like shift/scale");
+}
+
 void modulate_int8_quant(at::Tensor& out, at::Tensor& scales,
                          const std::optional<at::Tensor>& hidden_out, const at::Tensor& x,
                          const at::Tensor& shift, const at::Tensor& scale,
@@ -430,10 +464,7 @@ void rms_norm_modulate_int8_quant(at::Tensor& out, at::Tensor& scales,
                                   const at::Tensor& shift, const at::Tensor& scale,
                                   const std::optional<at::Tensor>& index) {
   const ModulateArgs r = check_modulate(out, scales, hidden_out, x, shift, scale, index);
-  check_cuda(weight, x, "weight");
-  TORCH_CHECK(weight.scalar_type() == at::kBFloat16 && weight.is_contiguous() &&
-                  weight.numel() == r.cols,
-              "norm weight must be contiguous bfloat16 [cols]");
+  check_norm_weight(weight, x, r.cols);
   const c10::cuda::CUDAGuard guard(x.device());
   check_status(tm_rms_norm_modulate_int8_quant(out.data_ptr<int8_t>(), scales.data_ptr<float>(),
                                                r.hidden, x.data_ptr(), weight.data_ptr(),
@@ -449,22 +480,8 @@ void residual_gate_rms_norm_modulate_int8_quant(
     const at::Tensor& branch, const at::Tensor& gate, const at::Tensor& weight, double eps,
     const at::Tensor& shift, const at::Tensor& scale, const std::optional<at::Tensor>& index) {
   const ModulateArgs r = check_modulate(out, scales, hidden_out, residual, shift, scale, index);
-  check_cuda(weight, residual, "weight");
-  check_cuda(branch, residual, "branch");
-  check_cuda(gate, residual, "gate");
-  check_cuda(residual_out, residual, "residual_out");
-  TORCH_CHECK(weight.scalar_type() == at::kBFloat16 && weight.is_contiguous() &&
-                  weight.numel() == r.cols,
-              "norm weight must be contiguous bfloat16 [cols]");
-  TORCH_CHECK(branch.scalar_type() == at::kBFloat16 && branch.is_contiguous() &&
-                  branch.sizes() == residual.sizes(),
-              "branch must be contiguous bfloat16 with the residual's shape");
-  TORCH_CHECK(residual_out.scalar_type() == at::kBFloat16 && residual_out.is_contiguous() &&
-                  residual_out.numel() == residual.numel(),
-              "residual_out must be contiguous bfloat16 with the residual's shape");
-  TORCH_CHECK(gate.scalar_type() == at::kBFloat16 && gate.sizes() == shift.sizes() &&
-                  gate.stride(1) == 1 && gate.stride(0) == shift.stride(0),
-              "gate must be a bfloat16 table shaped and strided like shift/scale");
+  check_norm_weight(weight, residual, r.cols);
+  check_residual_gate(residual_out, residual, branch, gate, shift);
   const c10::cuda::CUDAGuard guard(residual.device());
   check_status(tm_residual_gate_rms_norm_modulate_int8_quant(
                    out.data_ptr<int8_t>(), scales.data_ptr<float>(), residual_out.data_ptr(),
@@ -473,6 +490,240 @@ void residual_gate_rms_norm_modulate_int8_quant(
                    scale.data_ptr(), r.index, r.table_stride, r.rows, r.cols,
                    stream_of(residual)),
                "residual_gate_rms_norm_modulate_int8_quant");
+}
+
+// ---- 4-bit block formats ----
+// The format is the dtype of the block scales: float8_e4m3fn (TM_FP4_NV) or
+// float8_e8m0fnu (TM_FP4_MX).
+int fp4_format(const at::Tensor& block_scales, const char* name) {
+  const auto t = block_scales.scalar_type();
+  TORCH_CHECK(t == at::kFloat8_e4m3fn || t == at::kFloat8_e8m0fnu, name,
+              " must be float8_e4m3fn (blocks of 16) or float8_e8m0fnu (blocks of 32)");
+  return t == at::kFloat8_e4m3fn ? TM_FP4_NV : TM_FP4_MX;
+}
+
+// Block scales of a [rows, cols] tensor: the whole padded tile buffer.
+uint8_t* fp4_blocks(const at::Tensor& t, const at::Tensor& ref, int64_t rows, int64_t cols,
+                    int format, const char* name) {
+  check_cuda(t, ref, name);
+  TORCH_CHECK(fp4_format(t, name) == format, name, " must be in the other operand's format");
+  uint64_t bytes = 0;
+  TORCH_CHECK(tm_fp4_block_scales_size(rows, cols, format, &bytes) == TM_OK,
+              "4-bit rows must be a positive multiple of 32 elements wide, got ", cols);
+  TORCH_CHECK(t.is_contiguous() && static_cast<uint64_t>(t.numel()) == bytes, name,
+              " must be contiguous with ", bytes, " elements for [", rows, ", ", cols, "]");
+  return static_cast<uint8_t*>(t.data_ptr());
+}
+
+uint8_t* fp4_codes(const at::Tensor& q, const at::Tensor& ref, int64_t rows, int64_t cols,
+                   const char* name) {
+  check_cuda(q, ref, name);
+  TORCH_CHECK(q.scalar_type() == at::kByte && q.is_contiguous() && q.numel() == rows * (cols / 2),
+              name, " must be contiguous uint8 with two codes a byte");
+  return q.data_ptr<uint8_t>();
+}
+
+// Outer scales written by a quantising call: one a row (TM_FP4_NV), none (TM_FP4_MX).
+float* fp4_row_scales(const std::optional<at::Tensor>& scales, const at::Tensor& ref, int64_t rows,
+                      int format) {
+  if (!scales.has_value()) return nullptr;
+  check_cuda(*scales, ref, "scales");
+  TORCH_CHECK(format == TM_FP4_NV, "blocks of 32 take no fp32 scales");
+  TORCH_CHECK(scales->scalar_type() == at::kFloat && scales->is_contiguous() &&
+                  scales->numel() == rows,
+              "scales must be contiguous float32, one per row");
+  return scales->data_ptr<float>();
+}
+
+void scaled_fp4_quant(at::Tensor& q, at::Tensor& block_scales,
+                      const std::optional<at::Tensor>& scales, const at::Tensor& input,
+                      const std::optional<at::Tensor>& given_scale) {
+  check_cuda(input, input, "input");
+  const int dt = dtype_code(input);
+  TORCH_CHECK(dt >= 0, "input dtype must be bfloat16, float16 or float32");
+  int64_t rows, cols, ld;
+  as_rows(input, &rows, &cols, &ld);
+  const int format = fp4_format(block_scales, "block_scales");
+  uint8_t* blocks = fp4_blocks(block_scales, input, rows, cols, format, "block_scales");
+  uint8_t* codes = fp4_codes(q, input, rows, cols, "q");
+  float* row_scales = fp4_row_scales(scales, input, rows, format);
+  const float* given = nullptr;
+  if (given_scale.has_value()) {
+    check_cuda(*given_scale, input, "scale");
+    TORCH_CHECK(format == TM_FP4_NV, "blocks of 32 take no fp32 scale");
+    TORCH_CHECK(given_scale->scalar_type() == at::kFloat && given_scale->numel() == 1,
+                "a given scale must be one float32 value");
+    given = given_scale->data_ptr<float>();
+  }
+  TORCH_CHECK(format == TM_FP4_MX || scales.has_value() != given_scale.has_value(),
+              "blocks of 16 need either scales to write or a given scale");
+  const c10::cuda::CUDAGuard guard(input.device());
+  check_status(tm_scaled_fp4_quant(codes, blocks, row_scales, given, input.data_ptr(), dt, format,
+                                   rows, cols, ld, stream_of(input)),
+               "scaled_fp4_quant");
+}
+
+void dequantize_fp4(at::Tensor& out, const at::Tensor& q, const at::Tensor& block_scales,
+                    const std::optional<at::Tensor>& scales) {
+  check_cuda(q, q, "q");
+  check_cuda(out, q, "out");
+  const int dt = dtype_code(out);
+  TORCH_CHECK(dt >= 0, "out dtype must be bfloat16, float16 or float32");
+  TORCH_CHECK(out.dim() >= 1 && out.is_contiguous(), "out must be contiguous");
+  const int64_t cols = out.size(-1);
+  const int64_t rows = cols == 0 ? 0 : out.numel() / cols;
+  const int format = fp4_format(block_scales, "block_scales");
+  const uint8_t* blocks = fp4_blocks(block_scales, q, rows, cols, format, "block_scales");
+  const uint8_t* codes = fp4_codes(q, q, rows, cols, "q");
+  const float* s = nullptr;
+  if (scales.has_value()) {
+    check_cuda(*scales, q, "scales");
+    TORCH_CHECK(format == TM_FP4_NV, "blocks of 32 take no fp32 scales");
+    TORCH_CHECK(scales->scalar_type() == at::kFloat && scales->is_contiguous() &&
+                    (scales->numel() == 1 || scales->numel() == rows),
+                "scales must be contiguous float32, one or one per row");
+    s = scales->data_ptr<float>();
+  }
+  TORCH_CHECK(format == TM_FP4_MX || s != nullptr, "blocks of 16 need their fp32 scales");
+  const c10::cuda::CUDAGuard guard(q.device());
+  check_status(tm_dequantize_fp4(out.data_ptr(), dt, codes, blocks, s,
+                                 scales.has_value() ? scales->numel() : 0, format, rows, cols,
+                                 stream_of(q)),
+               "dequantize_fp4");
+}
+
+struct Fp4Out {
+  uint8_t* codes;
+  uint8_t* blocks;
+  float* scales;
+  int format;
+};
+
+Fp4Out check_fp4_out(const at::Tensor& q, const at::Tensor& block_scales,
+                     const std::optional<at::Tensor>& scales, const at::Tensor& x,
+                     const ModulateArgs& r) {
+  Fp4Out o;
+  o.format = fp4_format(block_scales, "block_scales");
+  o.blocks = fp4_blocks(block_scales, x, r.rows, r.cols, o.format, "block_scales");
+  o.codes = fp4_codes(q, x, r.rows, r.cols, "q");
+  o.scales = fp4_row_scales(scales, x, r.rows, o.format);
+  TORCH_CHECK(o.format == TM_FP4_MX || o.scales != nullptr, "blocks of 16 need scales to write");
+  return o;
+}
+
+void modulate_fp4_quant(at::Tensor& q, at::Tensor& block_scales,
+                        const std::optional<at::Tensor>& scales,
+                        const std::optional<at::Tensor>& hidden_out, const at::Tensor& x,
+                        const at::Tensor& shift, const at::Tensor& scale,
+                        const std::optional<at::Tensor>& index) {
+  const ModulateArgs r = check_modulate_inputs(hidden_out, x, shift, scale, index);
+  const Fp4Out o = check_fp4_out(q, block_scales, scales, x, r);
+  const c10::cuda::CUDAGuard guard(x.device());
+  check_status(tm_modulate_fp4_quant(o.codes, o.blocks, o.scales, r.hidden, x.data_ptr(),
+                                     shift.data_ptr(), scale.data_ptr(), r.index, r.table_stride,
+                                     o.format, r.rows, r.cols, stream_of(x)),
+               "modulate_fp4_quant");
+}
+
+void rms_norm_modulate_fp4_quant(at::Tensor& q, at::Tensor& block_scales,
+                                 const std::optional<at::Tensor>& scales,
+                                 const std::optional<at::Tensor>& hidden_out, const at::Tensor& x,
+                                 const at::Tensor& weight, double eps, const at::Tensor& shift,
+                                 const at::Tensor& scale, const std::optional<at::Tensor>& index) {
+  const ModulateArgs r = check_modulate_inputs(hidden_out, x, shift, scale, index);
+  const Fp4Out o = check_fp4_out(q, block_scales, scales, x, r);
+  check_norm_weight(weight, x, r.cols);
+  const c10::cuda::CUDAGuard guard(x.device());
+  check_status(tm_rms_norm_modulate_fp4_quant(o.codes, o.blocks, o.scales, r.hidden, x.data_ptr(),
+                                              weight.data_ptr(), static_cast<float>(eps),
+                                              shift.data_ptr(), scale.data_ptr(), r.index,
+                                              r.table_stride, o.format, r.rows, r.cols,
+                                              stream_of(x)),
+               "rms_norm_modulate_fp4_quant");
+}
+
+void residual_gate_rms_norm_modulate_fp4_quant(
+    at::Tensor& q, at::Tensor& block_scales, const std::optional<at::Tensor>& scales,
+    at::Tensor& residual_out, const std::optional<at::Tensor>& hidden_out,
+    const at::Tensor& residual, const at::Tensor& branch, const at::Tensor& gate,
+    const at::Tensor& weight, double eps, const at::Tensor& shift, const at::Tensor& scale,
+    const std::optional<at::Tensor>& index) {
+  const ModulateArgs r = check_modulate_inputs(hidden_out, residual, shift, scale, index);
+  const Fp4Out o = check_fp4_out(q, block_scales, scales, residual, r);
+  check_norm_weight(weight, residual, r.cols);
+  check_residual_gate(residual_out, residual, branch, gate, shift);
+  const c10::cuda::CUDAGuard guard(residual.device());
+  check_status(tm_residual_gate_rms_norm_modulate_fp4_quant(
+                   o.codes, o.blocks, o.scales, residual_out.data_ptr(), r.hidden,
+                   residual.data_ptr(), branch.data_ptr(), gate.data_ptr(), weight.data_ptr(),
+                   static_cast<float>(eps), shift.data_ptr(), scale.data_ptr(), r.index,
+                   r.table_stride, o.format, r.rows, r.cols, stream_of(residual)),
+               "residual_gate_rms_norm_modulate_fp4_quant");
+}
+
+const float* fp4_outer(const std::optional<at::Tensor>& t, const at::Tensor& ref, int64_t n,
+                       int format, const char* name) {
+  TORCH_CHECK(t.has_value() == (format == TM_FP4_NV), name,
+              format == TM_FP4_NV ? " is needed with blocks of 16" : " must be None with blocks of 32");
+  if (!t.has_value()) return nullptr;
+  check_cuda(*t, ref, name);
+  TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() &&
+                  (t->numel() == 1 || t->numel() == n),
+              name, " must be contiguous float32 with 1 or ", n, " values");
+  return t->data_ptr<float>();
+}
+
+void scaled_mm_fp4(at::Tensor& out, const at::Tensor& a, const at::Tensor& b,
+                   const at::Tensor& block_scales_a, const at::Tensor& block_scales_b,
+                   const std::optional<at::Tensor>& scales_a,
+                   const std::optional<at::Tensor>& scales_b,
+                   const std::optional<at::Tensor>& bias, int64_t epilogue, int64_t tile,
+                   int64_t splits) {
+  check_cuda(a, a, "a");
+  check_cuda(b, a, "b");
+  check_cuda(out, a, "out");
+  TORCH_CHECK(a.scalar_type() == at::kByte && b.scalar_type() == at::kByte,
+              "a and b must be uint8 (two codes a byte)");
+  TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && out.dim() == 2, "a, b and out must be 2-D");
+  const int64_t m = a.size(0), k = 2 * a.size(1), n = b.size(1);
+  TORCH_CHECK(2 * b.size(0) == k, "a and b inner dimensions differ: ", a.size(1), " vs ", b.size(0),
+              " bytes");
+  const int64_t out_n = (epilogue & TM_EPI_SWIGLU) ? n / 2 : n;
+  TORCH_CHECK(out.size(0) == m && out.size(1) == out_n, "out must be [", m, ", ", out_n, "]");
+  TORCH_CHECK(a.stride(1) == 1, "a must be row-major");
+  TORCH_CHECK(b.stride(0) == 1, "b must be column-major (pass weight.t())");
+  TORCH_CHECK(out.stride(1) == 1, "out must be row-major");
+  const int out_dt = dtype_code(out);
+  TORCH_CHECK(out_dt == TM_DTYPE_BF16 || out_dt == TM_DTYPE_FP16, "out must be bfloat16 or float16");
+  const int format = fp4_format(block_scales_a, "block_scales_a");
+  const uint8_t* blocks_a = fp4_blocks(block_scales_a, a, m, k, format, "block_scales_a");
+  const uint8_t* blocks_b = fp4_blocks(block_scales_b, a, n, k, format, "block_scales_b");
+  const float* sa = fp4_outer(scales_a, a, m, format, "scales_a");
+  const float* sb = fp4_outer(scales_b, a, n, format, "scales_b");
+  const void* bias_ptr = nullptr;
+  if (bias.has_value()) {
+    check_cuda(*bias, a, "bias");
+    TORCH_CHECK(bias->scalar_type() == out.scalar_type(), "bias must have the output dtype");
+    TORCH_CHECK(bias->numel() == n && bias->is_contiguous(), "bias must be contiguous [n]");
+    bias_ptr = bias->data_ptr();
+  }
+  const int64_t lda = m > 1 ? a.stride(0) : k / 2;
+  const int64_t ldb = n > 1 ? b.stride(1) : k / 2;
+  const int64_t ldo = m > 1 ? out.stride(0) : (out_n + 7) / 8 * 8;
+  const c10::cuda::CUDAGuard guard(a.device());
+  const int64_t na = scales_a.has_value() ? scales_a->numel() : 0;
+  const int64_t nb = scales_b.has_value() ? scales_b->numel() : 0;
+  const int status =
+      tile == 0 ? tm_scaled_mm_fp4(out.data_ptr(), out_dt, a.data_ptr<uint8_t>(),
+                                   b.data_ptr<uint8_t>(), blocks_a, blocks_b, sa, na, sb, nb,
+                                   bias_ptr, format, m, n, k, lda, ldb, ldo,
+                                   static_cast<uint32_t>(epilogue), stream_of(a))
+                : tm_scaled_mm_fp4_tile(out.data_ptr(), out_dt, a.data_ptr<uint8_t>(),
+                                        b.data_ptr<uint8_t>(), blocks_a, blocks_b, sa, na, sb, nb,
+                                        bias_ptr, format, m, n, k, lda, ldb, ldo,
+                                        static_cast<uint32_t>(epilogue), static_cast<int>(tile),
+                                        static_cast<int>(splits), stream_of(a));
+  check_status(status, "scaled_mm_fp4");
 }
 
 }  // namespace
@@ -504,6 +755,27 @@ TORCH_LIBRARY(taomate_w8a8, m) {
       "residual_gate_rms_norm_modulate_int8_quant(Tensor(a!) out, Tensor(b!) scales, "
       "Tensor(c!) residual_out, Tensor(d!)? hidden_out, Tensor residual, Tensor branch, "
       "Tensor gate, Tensor weight, float eps, Tensor shift, Tensor scale, Tensor? index) -> ()");
+  m.def(
+      "scaled_fp4_quant(Tensor(a!) q, Tensor(b!) block_scales, Tensor(c!)? scales, Tensor input, "
+      "Tensor? given_scale) -> ()");
+  m.def(
+      "dequantize_fp4(Tensor(a!) out, Tensor q, Tensor block_scales, Tensor? scales) -> ()");
+  m.def(
+      "modulate_fp4_quant(Tensor(a!) q, Tensor(b!) block_scales, Tensor(c!)? scales, "
+      "Tensor(d!)? hidden_out, Tensor x, Tensor shift, Tensor scale, Tensor? index) -> ()");
+  m.def(
+      "rms_norm_modulate_fp4_quant(Tensor(a!) q, Tensor(b!) block_scales, Tensor(c!)? scales, "
+      "Tensor(d!)? hidden_out, Tensor x, Tensor weight, float eps, Tensor shift, Tensor scale, "
+      "Tensor? index) -> ()");
+  m.def(
+      "residual_gate_rms_norm_modulate_fp4_quant(Tensor(a!) q, Tensor(b!) block_scales, "
+      "Tensor(c!)? scales, Tensor(d!) residual_out, Tensor(e!)? hidden_out, Tensor residual, "
+      "Tensor branch, Tensor gate, Tensor weight, float eps, Tensor shift, Tensor scale, "
+      "Tensor? index) -> ()");
+  m.def(
+      "scaled_mm_fp4(Tensor(a!) out, Tensor a, Tensor b, Tensor block_scales_a, "
+      "Tensor block_scales_b, Tensor? scales_a, Tensor? scales_b, Tensor? bias, int epilogue, "
+      "int tile, int splits) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(taomate_w8a8, CUDA, m) {
@@ -519,4 +791,10 @@ TORCH_LIBRARY_IMPL(taomate_w8a8, CUDA, m) {
   m.impl("rms_norm_modulate_int8_quant", &rms_norm_modulate_int8_quant);
   m.impl("residual_gate_rms_norm_modulate_int8_quant",
          &residual_gate_rms_norm_modulate_int8_quant);
+  m.impl("scaled_fp4_quant", &scaled_fp4_quant);
+  m.impl("dequantize_fp4", &dequantize_fp4);
+  m.impl("modulate_fp4_quant", &modulate_fp4_quant);
+  m.impl("rms_norm_modulate_fp4_quant", &rms_norm_modulate_fp4_quant);
+  m.impl("residual_gate_rms_norm_modulate_fp4_quant", &residual_gate_rms_norm_modulate_fp4_quant);
+  m.impl("scaled_mm_fp4", &scaled_mm_fp4);
 }

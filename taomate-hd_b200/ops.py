@@ -183,6 +183,122 @@ def lora_down_proj(x: torch.Tensor, a: torch.Tensor, *,
     return out
 
 
+_FP4_BLOCK_DTYPES = {"nvfp4": (16, torch.float8_e4m3fn), "mxfp4": (32, torch.float8_e8m0fnu)}
+
+
+def _empty_fp4(
+    like: torch.Tensor, block_format: str, row_scales: bool
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """Uninitialised ``(codes, block scales, row scales or None)`` for a tensor like ``like``."""
+    if block_format not in _FP4_BLOCK_DTYPES:
+        raise ValueError(f"block_format must be one of {sorted(_FP4_BLOCK_DTYPES)}")
+    block, dtype = _FP4_BLOCK_DTYPES[block_format]
+    cols = like.shape[-1] if like.dim() else 0
+    if cols == 0 or cols % 32:
+        raise ValueError(f"4-bit rows must be a positive multiple of 32 elements wide, got {cols}")
+    rows = like.numel() // cols
+    q = torch.empty((*like.shape[:-1], cols // 2), dtype=torch.uint8, device=like.device)
+    tiles = (-(-rows // 128) * 128, -(-(cols // block) // 4) * 4)
+    block_scales = torch.empty(tiles, dtype=torch.uint8, device=like.device).view(dtype)
+    scales = (torch.empty((rows, 1), dtype=torch.float32, device=like.device)
+              if row_scales and block_format == "nvfp4" else None)
+    return q, block_scales, scales
+
+
+def scaled_fp4_quant(
+    input: torch.Tensor,
+    scale: torch.Tensor | None = None,
+    *,
+    block_format: str = "nvfp4",
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """Quantise ``input`` (bf16, fp16 or fp32, last dimension a multiple of 32)
+    to 4 bits; returns ``(codes, block_scales, scales)``.
+
+    ``codes`` is uint8 ``[..., K / 2]``: two e2m1 codes a byte, the even
+    element in the low half.  ``block_scales`` holds one scale per block of a
+    row in the tiled order the tensor cores take (``include/taomate_w8a8.h``);
+    its dtype names the format:
+
+    * ``"nvfp4"``: blocks of 16 with an e4m3 scale, times an fp32 scale of
+      each row (``scales``, ``[rows, 1]``), or of the whole tensor when
+      ``scale`` (one fp32 value, the step between stored and real values) is
+      given; ``scales`` is then that tensor.
+    * ``"mxfp4"``: blocks of 32 with a power-of-two scale (e8m0); ``scales``
+      is ``None`` and no ``scale`` is taken.
+
+    Values are ``code * block scale * scale``; every rounding is to nearest,
+    ties to even, of the exact quotient.  Weights are converted by the same
+    call: their rows are the output channels.  A row (or block) that holds an
+    infinity or a NaN becomes NaN as a whole.
+    """
+    _require_cuda(input, scale)
+    q, block_scales, scales = _empty_fp4(input, block_format, scale is None)
+    if scale is not None and block_format != "nvfp4":
+        raise ValueError("only nvfp4 takes an fp32 scale")
+    x = input if input.dim() == 2 and input.stride(1) == 1 else input.contiguous()
+    _ops.scaled_fp4_quant(q, block_scales, scales, x, scale)
+    return q, block_scales, scales if scale is None else scale
+
+
+def dequantize_fp4(
+    q: torch.Tensor,
+    block_scales: torch.Tensor,
+    scales: torch.Tensor | None = None,
+    out_dtype: torch.dtype = torch.bfloat16,
+) -> torch.Tensor:
+    """The values of a tensor quantised by :func:`scaled_fp4_quant`, ``[..., K]``
+    in ``out_dtype`` (bf16, fp16 or fp32): what a layer would see at 4 bits."""
+    _require_cuda(q, block_scales, scales)
+    out = torch.empty((*q.shape[:-1], 2 * q.shape[-1]), dtype=out_dtype, device=q.device)
+    _ops.dequantize_fp4(out, q.contiguous(), block_scales, scales)
+    return out
+
+
+def scaled_mm_fp4(
+    a: torch.Tensor,
+    b: torch.Tensor,
+    block_scale_a: torch.Tensor,
+    block_scale_b: torch.Tensor,
+    scale_a: torch.Tensor | None = None,
+    scale_b: torch.Tensor | None = None,
+    out_dtype: torch.dtype = torch.bfloat16,
+    bias: torch.Tensor | None = None,
+    *,
+    gelu_tanh: bool = False,
+    swiglu: bool = False,
+    out: torch.Tensor | None = None,
+    tile: int = 0,
+    splits: int = 1,
+) -> torch.Tensor:
+    """Product of two 4-bit tensors of the same block format: the linear
+    ``act(x @ w.T (+ bias))`` of their values, ``[..., N]`` in ``out_dtype``.
+
+    ``a``: uint8 codes ``[..., K / 2]``; ``b``: uint8 ``[K / 2, N]``
+    column-major (the ``.t()`` view of the weight's codes); the block scales
+    and fp32 scales as :func:`scaled_fp4_quant` returns them (``None`` for
+    mxfp4).  ``N`` must be a multiple of 8.  ``gelu_tanh`` and ``swiglu``
+    (interleaved gate/up rows, :func:`interleave_gate_up`) as in
+    :func:`scaled_mm`, except that the result is rounded once, after the
+    activation.  ``out`` ([M, N] or [M, N / 2]) makes the call allocation-free;
+    ``tile`` and ``splits`` force a kernel configuration (0 = heuristic).
+    """
+    _require_cuda(a, b, block_scale_a, block_scale_b, scale_a, scale_b, bias, out)
+    if gelu_tanh and swiglu:
+        raise ValueError("gelu_tanh and swiglu are exclusive")
+    if a.dim() == 0 or a.shape[-1] == 0:
+        raise ValueError("a must be [..., K / 2] with K > 0")
+    a2 = a if a.dim() == 2 else a.reshape(-1, a.shape[-1])
+    shape = None
+    if out is None:
+        cols = b.shape[1] // 2 if swiglu else b.shape[1]
+        shape = (*a.shape[:-1], cols)
+        out = torch.empty((a2.shape[0], cols), dtype=out_dtype, device=a.device)
+    epi = (EPI_GELU_TANH if gelu_tanh else 0) | (EPI_SWIGLU if swiglu else 0)
+    _ops.scaled_mm_fp4(out, a2, b, block_scale_a, block_scale_b, scale_a, scale_b, bias, epi, tile,
+                       splits)
+    return out if shape is None else out.view(shape)
+
+
 def quantize_weight_int8(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Per-output-channel symmetric int8 weight conversion on the GPU.
 
@@ -333,3 +449,68 @@ def residual_gate_rms_norm_modulate_int8_quant(
     _ops.residual_gate_rms_norm_modulate_int8_quant(
         q, s, residual_out, hidden, residual, branch, gate, weight, float(eps), shift, scale, index)
     return q, s, residual_out, hidden
+
+
+def modulate_fp4_quant(
+    x: torch.Tensor,
+    shift: torch.Tensor,
+    scale: torch.Tensor,
+    index: torch.Tensor | None = None,
+    *,
+    block_format: str = "nvfp4",
+    return_hidden: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
+    """:func:`modulate_int8_quant` with 4-bit output: returns ``(codes,
+    block_scales, scales or None, hidden or None)``, the hidden state the same
+    bits as the int8 producer's, quantised as by :func:`scaled_fp4_quant`."""
+    _require_cuda(x, shift, scale, index)
+    q, b, s = _empty_fp4(x, block_format, True)
+    hidden = torch.empty_like(x) if return_hidden else None
+    _ops.modulate_fp4_quant(q, b, s, hidden, x, shift, scale, index)
+    return q, b, s, hidden
+
+
+def rms_norm_modulate_fp4_quant(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    eps: float,
+    shift: torch.Tensor,
+    scale: torch.Tensor,
+    index: torch.Tensor | None = None,
+    *,
+    block_format: str = "nvfp4",
+    return_hidden: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
+    """:func:`rms_norm_modulate_int8_quant` with 4-bit output
+    (:func:`modulate_fp4_quant`)."""
+    _require_cuda(x, weight, shift, scale, index)
+    q, b, s = _empty_fp4(x, block_format, True)
+    hidden = torch.empty_like(x) if return_hidden else None
+    _ops.rms_norm_modulate_fp4_quant(q, b, s, hidden, x, weight, float(eps), shift, scale, index)
+    return q, b, s, hidden
+
+
+def residual_gate_rms_norm_modulate_fp4_quant(
+    residual: torch.Tensor,
+    branch: torch.Tensor,
+    gate: torch.Tensor,
+    weight: torch.Tensor,
+    eps: float,
+    shift: torch.Tensor,
+    scale: torch.Tensor,
+    index: torch.Tensor | None = None,
+    *,
+    block_format: str = "nvfp4",
+    return_hidden: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None, torch.Tensor, torch.Tensor | None]:
+    """:func:`residual_gate_rms_norm_modulate_int8_quant` with 4-bit output:
+    returns ``(codes, block_scales, scales or None, updated residual, hidden
+    or None)``."""
+    _require_cuda(residual, branch, gate, weight, shift, scale, index)
+    q, b, s = _empty_fp4(residual, block_format, True)
+    residual_out = torch.empty_like(residual)
+    hidden = torch.empty_like(residual) if return_hidden else None
+    _ops.residual_gate_rms_norm_modulate_fp4_quant(
+        q, b, s, residual_out, hidden, residual, branch, gate, weight, float(eps), shift, scale,
+        index)
+    return q, b, s, residual_out, hidden

@@ -1,0 +1,285 @@
+"""GPU parity of the 4-bit operators against the 64-bit restatement (oracle/fp4_oracle.py).
+
+Codes, block scales, row scales and the producers' hidden states are held to
+every bit.  Products: with S = sum |va vb| (outer scales included), the fp32
+accumulation of K products in groups of at most a block adds at most
+(K / 16 + 16) 2^-23 S (one step per block and per alignment inside a group),
+and the output rounding half a step, finfo.eps / 2 of the value.  The GELU
+multiplies the first by at most 1.13 and adds the tanh instruction's 2^-11 of
+|y| / 2; SwiGLU's sigmoid costs (2 + |g|) 2^-22 of the value (exponential and
+quotient to 2 units each).
+"""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import fp4_oracle as f4
+from oracle import w8a8_oracle as orc
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = ("nvfp4", "mxfp4")
+HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+
+
+def _check_quant(got, x, fmt, given=None):
+    q, blocks, scales = got
+    q_ref, b_ref, s_ref = f4.quantise(x.reshape(-1, x.shape[-1]), fmt, given)
+    np.testing.assert_array_equal(blocks.view(torch.uint8).cpu().numpy(), b_ref)
+    np.testing.assert_array_equal(q.cpu().numpy().reshape(q_ref.shape), q_ref)
+    if fmt == "nvfp4" and given is None:
+        np.testing.assert_array_equal(scales.cpu().numpy().reshape(-1), s_ref)
+        assert scales.shape == (s_ref.size, 1)
+    if fmt == "mxfp4":
+        assert scales is None
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize(
+    "rows,cols",
+    [(1, 32), (3, 64), (7, 96), (33, 160), (130, 1376), (257, 2688), (5, 5376), (2, 12288),
+     (1, 20000), (2, 33024)],
+)
+def test_quant_bit_exact(tm_ops, cuda, rows, cols, dtype, fmt):
+    x = orc.activation(rows, cols, rows * 7919 + cols, outlier_channels=None).to(dtype)
+    got = tm_ops.scaled_fp4_quant(x.to(cuda), block_format=fmt)
+    assert got[0].shape == (rows, cols // 2) and got[0].dtype == torch.uint8
+    assert got[1].dtype == (torch.float8_e4m3fn if fmt == "nvfp4" else torch.float8_e8m0fnu)
+    _check_quant(got, x, fmt)
+
+
+def _borders(dtype):
+    """Rows whose elements sit on, just below and just above the code borders
+    of scales with every mantissa, and rows of extremes."""
+    rows = []
+    for mantissa in range(8):
+        s = 1.0 + mantissa / 8
+        for top in (6.0, 5.0, 4.5):
+            t = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], dtype=torch.float64)
+            step = torch.finfo(dtype).eps
+            near = torch.cat((t, t * (1 + step), t * (1 - step)))
+            row = torch.zeros(64, dtype=torch.float64)
+            row[:21] = near * s
+            row[21] = -top * s
+            row[32:53] = -near * s * 0.5
+            row[63] = 2.0 ** (mantissa - 4)
+            rows.append(row)
+    x = torch.stack(rows)
+    x = torch.cat((x, x * 0.1, x * 448, x * (1 / 3)), 0)
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_quant_on_the_borders(tm_ops, cuda, dtype, fmt):
+    x = _borders(dtype)
+    _check_quant(tm_ops.scaled_fp4_quant(x.to(cuda), block_format=fmt), x, fmt)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("given", [1.0, 1 / 3, 0.0371, 90.0 / 2688, 1000.0, 1e-5])
+def test_quant_given_scale(tm_ops, cuda, dtype, given):
+    x = torch.cat((_borders(dtype), orc.activation(9, 64, 3, outlier_channels=None).to(dtype)))
+    scale = torch.tensor([given], device=cuda)
+    got = tm_ops.scaled_fp4_quant(x.to(cuda), scale)
+    assert got[2] is scale
+    _check_quant(got, x, "nvfp4", given)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_quant_extreme_rows(tm_ops, cuda, dtype, fmt):
+    x = torch.randn(12, 512, generator=torch.Generator().manual_seed(1))
+    x[0] = 0.0
+    x[1] = -0.0
+    x[2] *= 1e-40  # subnormal
+    x[3] *= 1e-35
+    x[4] *= 1e38
+    x[5, 7] = float("inf")
+    x[6, 100] = float("-inf")
+    x[7, 511] = float("nan")
+    x[8, :] = 0.0
+    x[8, 5] = 3.0  # one block in use
+    x[9, :16] *= 1e-6  # blocks whose scale underflows to 0
+    x[10] = torch.finfo(dtype).max
+    x[11] = torch.finfo(dtype).tiny
+    x = x.to(dtype)
+    got = tm_ops.scaled_fp4_quant(x.to(cuda), block_format=fmt)
+    _check_quant(got, x, fmt)
+    if fmt == "nvfp4":
+        assert torch.isnan(got[2][5:8]).all()
+        _check_quant(tm_ops.scaled_fp4_quant(x.to(cuda), torch.tensor([0.01], device=cuda)), x, fmt,
+                     0.01)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quant_strides_and_alignment(tm_ops, cuda, fmt):
+    big = orc.activation(40, 1024, 6, outlier_channels=None).bfloat16().to(cuda)
+    for view in (big[:, :512], big[:, 8:520], big[:, 16:528], big[3:, 1:129], big[::2, :96],
+                 big.reshape(8, 5, 1024), big.t()[:, :32], big[:, ::2]):
+        _check_quant(tm_ops.scaled_fp4_quant(view, block_format=fmt), view.cpu().contiguous(), fmt)
+    f = big.float()
+    for view in (f[:, 4:516], f[:, 1:65]):
+        _check_quant(tm_ops.scaled_fp4_quant(view, block_format=fmt), view.cpu().contiguous(), fmt)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quant_rows_behind_the_last_are_left(tm_ops, cuda, fmt):
+    x = orc.activation(130, 96, 2, outlier_channels=None).bfloat16().to(cuda)
+    q = torch.full((140, 48), 0xAB, dtype=torch.uint8, device=cuda)
+    blocks = torch.empty_like(tm_ops.scaled_fp4_quant(x, block_format=fmt)[1])
+    s = torch.full((140, 1), 7.0, device=cuda)
+    torch.ops.taomate_w8a8.scaled_fp4_quant(q[:130], blocks, s[:130] if fmt == "nvfp4" else None, x,
+                                            None)
+    assert (q[130:] == 0xAB).all() and (s[130:] == 7.0).all()
+    empty = tm_ops.scaled_fp4_quant(x[:0], block_format=fmt)
+    assert empty[0].shape == (0, 48) and empty[1].numel() == 0
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,cols", [(1, 32), (130, 1376), (3, 20000)])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_dequantise(tm_ops, cuda, rows, cols, out_dtype, fmt):
+    x = orc.activation(rows, cols, rows + cols, outlier_channels=None).bfloat16()
+    q, b, s = tm_ops.scaled_fp4_quant(x.to(cuda), block_format=fmt)
+    got = tm_ops.dequantize_fp4(q, b, s, out_dtype).cpu().double().numpy()
+    ref = f4.stored_values(q.cpu().numpy(), b.view(torch.uint8).cpu().numpy(), fmt)
+    if s is not None:
+        ref = ref * s.cpu().double().numpy()
+    # one fp32 rounding of the product with the row scale, one to the output
+    tol = np.abs(ref) * (HALF_STEP[out_dtype] + 2.0 ** -24) * (1 + 2.0 ** -8)
+    if out_dtype == torch.float16:
+        tol = tol + 2.0 ** -25  # half a subnormal step
+    assert (np.abs(got - ref) <= tol).all()
+
+
+def test_dequantise_given_scale_and_nan(tm_ops, cuda):
+    x = torch.randn(4, 64, generator=torch.Generator().manual_seed(3))
+    x[1, 3] = float("nan")
+    x[2, 40] = float("inf")
+    scale = torch.tensor([0.01], device=cuda)
+    y = tm_ops.dequantize_fp4(*tm_ops.scaled_fp4_quant(x.to(cuda), scale))
+    assert torch.isnan(y[1, :16]).all() and torch.isfinite(y[1, 16:]).all()
+    assert torch.isnan(y[2, 32:48]).all() and torch.isfinite(y[2, :32]).all()
+    y = tm_ops.dequantize_fp4(*tm_ops.scaled_fp4_quant(x.to(cuda)))
+    assert torch.isnan(y[1:3]).all() and torch.isfinite(y[0]).all() and torch.isfinite(y[3]).all()
+    y = tm_ops.dequantize_fp4(*tm_ops.scaled_fp4_quant(x.to(cuda), block_format="mxfp4"))
+    assert torch.isnan(y[1, :32]).all() and torch.isfinite(y[1, 32:]).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,cols,tables", [(1, 32, 0), (130, 1376, 3), (37, 3072, 0), (5, 5376, 2),
+                                              (2, 20480, 1)])
+@pytest.mark.parametrize("mode", ["modulate", "rms", "residual"])
+def test_producers(tm_ops, cuda, mode, rows, cols, tables, fmt):
+    """The hidden state and residual are the int8 producers' bits, and the
+    codes those of the plain quantisation of that hidden state."""
+    g = torch.Generator().manual_seed(rows + cols)
+    rnd = lambda *shape, std=1.0: (torch.randn(shape, generator=g) * std).bfloat16().to(cuda)  # noqa: E731
+    x, branch = rnd(rows, cols), rnd(rows, cols)
+    shift, scale, gate = (rnd(tables or rows, cols, std=0.3) for _ in range(3))
+    index = torch.randint(0, tables, (rows,), generator=g).to(cuda) if tables else None
+    w = rnd(cols)
+    if mode == "modulate":
+        *got, hidden = tm_ops.modulate_fp4_quant(x, shift, scale, index, block_format=fmt,
+                                                 return_hidden=True)
+        ref = tm_ops.modulate_int8_quant(x, shift, scale, index, return_hidden=True)[-1]
+    elif mode == "rms":
+        *got, hidden = tm_ops.rms_norm_modulate_fp4_quant(x, w, 1e-6, shift, scale, index,
+                                                          block_format=fmt, return_hidden=True)
+        ref = tm_ops.rms_norm_modulate_int8_quant(x, w, 1e-6, shift, scale, index,
+                                                  return_hidden=True)[-1]
+    else:
+        *got, res, hidden = tm_ops.residual_gate_rms_norm_modulate_fp4_quant(
+            x, branch, gate, w, 1e-6, shift, scale, index, block_format=fmt, return_hidden=True)
+        _, _, res_ref, ref = tm_ops.residual_gate_rms_norm_modulate_int8_quant(
+            x, branch, gate, w, 1e-6, shift, scale, index, return_hidden=True)
+        assert torch.equal(res, res_ref)
+    assert torch.equal(hidden, ref)
+    _check_quant(got, hidden.cpu(), fmt)
+    if mode == "modulate":  # without the hidden state
+        again = tm_ops.modulate_fp4_quant(x, shift, scale, index, block_format=fmt)
+        assert again[3] is None and torch.equal(again[0], got[0])
+
+
+# ---------------------------------------------------------------- product
+def _operands(tm_ops, cuda, m, n, k, fmt, dtype, seed):
+    x = orc.activation(m, k, seed, outlier_channels=None).bfloat16().to(cuda)
+    w = orc.weight(n, k, seed=seed + 1).to(cuda)
+    g = torch.Generator().manual_seed(seed + 2)
+    bias = (torch.randn(n, generator=g) * 0.3).to(dtype).to(cuda)
+    return (*tm_ops.scaled_fp4_quant(x, block_format=fmt),
+            *tm_ops.scaled_fp4_quant(w, block_format=fmt), bias)
+
+
+def _values(q, b, s, fmt):
+    v = f4.stored_values(q.cpu().numpy(), b.view(torch.uint8).cpu().numpy(), fmt)
+    return v if s is None else v * s.cpu().double().numpy().reshape(-1, 1)
+
+
+def _check_mm(out, aq, ab, asc, wq, wb, wsc, bias, fmt, act="none"):
+    a, b = (torch.from_numpy(_values(*t, fmt)).to(out.device) for t in ((aq, ab, asc), (wq, wb, wsc)))
+    k = a.shape[1]
+    y = (a @ b.t()).cpu().numpy()
+    size = (a.abs() @ b.abs().t()).cpu().numpy()
+    slack = (k / 16 + 16) * 2.0 ** -23 * size
+    if bias is not None:
+        y = y + bias.cpu().double().numpy()
+        slack = slack + 2.0 ** -23 * np.abs(y)
+    half = HALF_STEP[out.dtype]
+    if act == "gelu":
+        ref = f4.gelu_tanh(y)
+        tol = 1.13 * slack + np.abs(y) / 2 * 2.0 ** -11
+    elif act == "swiglu":
+        ref = f4.swiglu(y)
+        p, s = y.reshape(y.shape[0], -1, 2, 16), slack.reshape(y.shape[0], -1, 2, 16)
+        g, u = p[:, :, 0], p[:, :, 1]
+        # d(g sigmoid(g)) <= 1.1 dg; |g sigmoid(g)| <= |g|
+        tol = (1.1 * s[:, :, 0] * (np.abs(u) + s[:, :, 1]) + np.abs(g) * s[:, :, 1]).reshape(ref.shape)
+        tol = tol + np.abs(ref) * (2 + np.abs(g).reshape(ref.shape)) * 2.0 ** -22
+    else:
+        ref, tol = y, slack
+    tol = tol + half * (np.abs(ref) + tol)
+    if out.dtype == torch.float16:
+        tol = tol + 2.0 ** -25
+    err = np.abs(out.cpu().double().numpy() - ref)
+    assert (err <= tol).all(), (float((err / tol).max()), np.argwhere(err > tol)[:4], err.max())
+
+
+SMALL = [(32, 1), (32, 2), (32, 4), (32, 8), (64, 1), (64, 4), (128, 1), (128, 2), (128, 8)]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tile,splits", SMALL)
+@pytest.mark.parametrize("m,n,k", [(1, 128, 2048), (31, 200, 2336), (17, 8, 2592), (32, 1160, 2048 + 96)])
+def test_mm_small_tiles(tm_ops, cuda, m, n, k, tile, splits, fmt):
+    *ops, bias = _operands(tm_ops, cuda, m, n, k, fmt, torch.bfloat16, m + n + k)
+    aq, ab, asc, wq, wb, wsc = ops
+    out = tm_ops.scaled_mm_fp4(aq, wq.t(), ab, wb, asc, wsc, bias=bias, tile=tile, splits=splits)
+    _check_mm(out, *ops, bias, fmt)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("k", [32, 64, 96, 128, 160, 224, 256, 288, 512, 1376])
+def test_mm_every_k_tail(tm_ops, cuda, k, dtype, fmt):
+    *ops, bias = _operands(tm_ops, cuda, 70, 136, k, fmt, dtype, k)
+    aq, ab, asc, wq, wb, wsc = ops
+    _check_mm(tm_ops.scaled_mm_fp4(aq, wq.t(), ab, wb, asc, wsc, dtype), *ops, None, fmt)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("act", ["none", "gelu", "swiglu"])
+@pytest.mark.parametrize("m,n,k", [(1, 64, 256), (60, 704, 1024), (300, 1344, 800), (1003, 1152, 1376)])
+def test_mm_epilogues(tm_ops, cuda, m, n, k, act, fmt):
+    *ops, bias = _operands(tm_ops, cuda, m, n, k, fmt, torch.bfloat16, m + n)
+    aq, ab, asc, wq, wb, wsc = ops
+    for b in (None, bias):
+        out = tm_ops.scaled_mm_fp4(aq, wq.t(), ab, wb, asc, wsc, bias=b, gelu_tanh=act == "gelu",
+                                   swiglu=act == "swiglu")
+        _check_mm(out, *ops, b, fmt, act)
