@@ -14,6 +14,12 @@
 // buffers alternate; one is written again only after the MMAs that read it
 // have completed.
 //
+//   gemm_fp4_pair_kernel  persistent CTA pairs (clusters of 2), a 256 token x 256
+//     weight row tile each: a CTA fetches 128 token rows and 128 weight rows, the
+//     leader issues tcgen05.mma.cta_group::2 (M = 256, N = 256), and each CTA's
+//     TMEM receives 128 x 256 sums.  Two such accumulators and the scales exceed
+//     the 512 TMEM columns, so the accumulators overlap by 128: an epilogue first
+//     takes the shared columns into registers, then lets the next tile start.
 //   gemm_fp4_small_kernel  one CTA per (128 weight rows x TOK tokens, K slice).
 //     The weight is the M operand (128 TMEM lanes), the tokens the N operand, so
 //     one token costs a 32-column accumulator and the weight streams once.
@@ -362,6 +368,374 @@ __global__ void __launch_bounds__(kSmallThreads)
   }
 }
 
+// ====================================================================== pair
+constexpr int kPairThreads = 320;  // producer, MMA, eight epilogue warps
+constexpr int kPairEpiWarps = 8;
+constexpr int kPairRows = 256;     // tokens, and weight rows, of a tile
+constexpr int kPairStages = 5;
+// per epilogue warp: a staging tile, 128 column scales and 128 bias values
+constexpr int kPairScaleCache = kStage64Bytes;
+constexpr int kPairBiasCache = kPairScaleCache + 512;
+constexpr int kPairRegion = 4096;
+
+template <int FORMAT>
+struct PairLayout {
+  using S = ScaleGeom<FORMAT>;
+  static constexpr int kHalfBytes = 128 * kRowBytes;
+  static constexpr int kStageBytes = 2 * kHalfBytes + 3 * S::kBytes;  // per CTA
+  static constexpr int kBarOffset = kPairStages * kStageBytes;
+  static constexpr int kEpiOffset = (kBarOffset + 256 + 1023) / 1024 * 1024;
+  static constexpr int kTotal = kEpiOffset + kPairEpiWarps * kPairRegion + 1024;
+  static_assert(kStageBytes % 1024 == 0, "stages stay aligned");
+  static_assert(kTotal <= 227 * 1024, "shared memory budget");
+  // TMEM: accumulator b at columns [128 b, 128 b + 256), scale buffers behind
+  static constexpr uint32_t kAccStep = 128;
+  static constexpr uint32_t kScaleCol = 384;
+  static constexpr uint32_t kScaleBuf = 3 * 4 * S::kTiles;
+  static_assert(kScaleCol + 2 * kScaleBuf <= 512, "TMEM columns");
+};
+
+struct PairBars {
+  uint64_t* full;
+  uint64_t* empty;
+  uint64_t* acc_full;
+  uint64_t* acc_free;
+  uint32_t* tmem_slot;
+  volatile int* abort_flag;
+};
+
+__device__ __forceinline__ PairBars pair_bars(uint8_t* base) {
+  PairBars b;
+  b.full = reinterpret_cast<uint64_t*>(base);
+  b.empty = b.full + kPairStages;
+  b.acc_full = b.empty + kPairStages;
+  b.acc_free = b.acc_full + 1;
+  b.tmem_slot = reinterpret_cast<uint32_t*>(b.acc_free + 1);
+  b.abort_flag = reinterpret_cast<volatile int*>(b.tmem_slot + 1);
+  return b;
+}
+
+// A lane's share of a tile's constants: four columns' scales and bias values
+// and its row's scale.  Columns of piece p (lane / 16): 128 p + 64 h + 4 (lane % 16).
+struct PairConsts {
+  float sb[4];
+  float bias[4];
+  float sa;
+};
+
+template <int FORMAT, typename OutT>
+__device__ __forceinline__ PairConsts pair_consts(const Fp4Args& g, int nb, int h, int64_t row,
+                                                  int lane) {
+  PairConsts c;
+  const int col = nb * kPairRows + 128 * (lane >> 4) + 64 * h + 4 * (lane & 15);
+  const bool in = col < g.N;  // N % 8 == 0: all four or none
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    c.sb[j] = FORMAT == TM_FP4_NV && in ? __ldg(g.sb + (g.sb_per_col ? col + j : 0)) : 0.f;
+    c.bias[j] =
+        g.bias != nullptr && in ? out_to_f32<OutT>(static_cast<const OutT*>(g.bias)[col + j]) : 0.f;
+  }
+  c.sa = FORMAT == TM_FP4_NV && row < g.M ? __ldg(g.sa + (g.sa_per_row ? row : 0)) : 1.f;
+  return c;
+}
+
+template <int FORMAT, typename OutT>
+__device__ __forceinline__ void pair_consts_store(uint8_t* region, const PairConsts& c, int lane) {
+  if constexpr (FORMAT == TM_FP4_NV)
+    *reinterpret_cast<float4*>(region + kPairScaleCache + 16 * lane) =
+        make_float4(c.sb[0], c.sb[1], c.sb[2], c.sb[3]);
+  *reinterpret_cast<uint2*>(region + kPairBiasCache + 8 * lane) =
+      make_uint2(pack2<OutT>(c.bias[0], c.bias[1]), pack2<OutT>(c.bias[2], c.bias[3]));
+}
+
+// Outer scales and bias on 32 accumulator columns (in place).
+template <int FORMAT, typename OutT>
+__device__ __forceinline__ void pair_scale32(const Fp4Args& g, uint32_t (&r)[32], float sa,
+                                             const float* sb, const OutT* bias) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 8) {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(r[j + i]);
+    if constexpr (FORMAT == TM_FP4_NV) {
+      const float4 s0 = *reinterpret_cast<const float4*>(sb + j);
+      const float4 s1 = *reinterpret_cast<const float4*>(sb + j + 4);
+      const float sc[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(sc[i], y[i]);
+    }
+    if (g.bias != nullptr) {
+      const uint4 b = *reinterpret_cast<const uint4*>(bias + j);
+      const OutT* e = reinterpret_cast<const OutT*>(&b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = __fmaf_rn(sa, y[i], out_to_f32<OutT>(e[i]));
+    } else if constexpr (FORMAT == TM_FP4_NV) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(sa, y[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[j + i] = __float_as_uint(y[i]);
+  }
+}
+
+// Stage 32 rows x 32 columns (a row per lane) and store them by TMA.
+template <typename OutT>
+__device__ __forceinline__ void pair_store32(const CUtensorMap* tm_out, uint8_t* region,
+                                             const float (&y)[32], int x, int64_t row, bool in,
+                                             int lane) {
+  if (lane == 0) bulk_wait_read_all();  // the previous store has left the tile
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    *stage64_slot(region, lane, j) =
+        make_uint4(pack2<OutT>(y[8 * j], y[8 * j + 1]), pack2<OutT>(y[8 * j + 2], y[8 * j + 3]),
+                   pack2<OutT>(y[8 * j + 4], y[8 * j + 5]), pack2<OutT>(y[8 * j + 6], y[8 * j + 7]));
+  fence_async_shared();
+  __syncwarp();
+  if (lane == 0 && in) {
+    tma_store_2d(tm_out, region, x, static_cast<int>(row));
+    bulk_commit();
+  }
+}
+
+template <int FORMAT, typename OutT>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
+                         const __grid_constant__ CUtensorMap tm_b,
+                         const __grid_constant__ CUtensorMap tm_as,
+                         const __grid_constant__ CUtensorMap tm_bs,
+                         const __grid_constant__ CUtensorMap tm_out, const Fp4Args g) {
+  using L = PairLayout<FORMAT>;
+  using S = ScaleGeom<FORMAT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1k(smem_raw);
+  const PairBars bar = pair_bars(smem + L::kBarOffset);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();  // 0 = leader (issues the MMAs)
+  const bool leader = rank == 0;
+  const int tiles = g.num_m * g.num_n;
+  const int pair = blockIdx.x >> 1;
+  const int pairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&bar.full[s], 1);
+      mbar_init(&bar.empty[s], 1);
+    }
+    mbar_init(bar.acc_full, 1);
+    mbar_init(bar.acc_free, 2 * kPairEpiWarps);  // both CTAs' epilogue warps
+    *bar.abort_flag = 0;
+    fence_mbarrier_init();
+    tma_prefetch_desc(&tm_a);
+    tma_prefetch_desc(&tm_b);
+    tma_prefetch_desc(&tm_as);
+    tma_prefetch_desc(&tm_bs);
+    tma_prefetch_desc(&tm_out);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(bar.tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();  // barriers of both CTAs initialised, TMEM allocated
+  tc_fence_after();
+  const uint32_t tmem_base = *bar.tmem_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t issued_mask = 0, issued_parity = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < tiles; tile += pairs) {
+        int mb, nb;
+        tile_coords(tile, g.num_m, g.num_n, mb, nb, 0, 0, g.group_n);
+        for (int kb = 0; kb < g.kblocks; ++kb) {
+          if (!mbar_wait(&bar.empty[stage], phase ^ 1u, bar.abort_flag, g.status)) {
+            ok = false;
+            break;
+          }
+          issued_mask &= ~(1u << stage);
+          uint8_t* s = smem + stage * L::kStageBytes;
+          uint8_t* scales = s + 2 * L::kHalfBytes;
+          // the leader's `full` barrier counts the bytes landing in both CTAs
+          if (leader) mbar_arrive_expect_tx(&bar.full[stage], 2 * L::kStageBytes);
+          const uint32_t full = map_to_cta(smem_u32(&bar.full[stage]), 0);
+          tma_load_2d_pair(&tm_a, full, s, kb * kRowBytes, mb * kPairRows + static_cast<int>(rank) * 128);
+          tma_load_2d_pair(&tm_b, full, s + L::kHalfBytes, kb * kRowBytes,
+                           nb * kPairRows + static_cast<int>(rank) * 128);
+          // own tokens' scales, and the whole tile's weight scales in both CTAs
+          tma_load_2d_pair(&tm_as, full, scales, kb * (S::kBytes / 8), mb * 2 + static_cast<int>(rank));
+          tma_load_2d_pair(&tm_bs, full, scales + S::kBytes, kb * (S::kBytes / 8), nb * 2);
+          issued_mask |= 1u << stage;
+          issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
+          if (++stage == kPairStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok) {
+        if (leader) {
+          for (int s = 0; s < kPairStages; ++s)
+            if (issued_mask & (1u << s))
+              mbar_wait_drain(&bar.full[s], (issued_parity >> s) & 1u, g.status);
+        } else {
+          // this CTA's copies complete on the leader's barriers, which it cannot
+          // poll; give any in-flight copy ample time to land
+          const uint64_t t0 = globaltimer_ns();
+          while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (leader && lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int last = -1, before = -1;  // stages of the previous k-block and of the one before it
+      uint32_t last_phase = 0, before_phase = 0;
+      uint32_t buf = 0;  // scale buffer
+      bool ok = true;
+      int i = 0;
+      for (int tile = pair; ok && tile < tiles; tile += pairs, ++i) {
+        // the previous tile's epilogue holds the columns the accumulators share
+        // (and has finished with everything before)
+        if (i > 0 && !mbar_wait(bar.acc_free, (i - 1) & 1, bar.abort_flag, g.status)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + (i & 1) * L::kAccStep;
+        for (int kb = 0; kb < g.kblocks; ++kb) {
+          // the scale buffer was last read two k-blocks ago
+          if ((before >= 0 &&
+               !mbar_wait(&bar.empty[before], before_phase, bar.abort_flag, g.status)) ||
+              !mbar_wait(&bar.full[stage], phase, bar.abort_flag, g.status)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(smem + stage * L::kStageBytes);
+          const uint32_t b_addr = a_addr + L::kHalfBytes;
+          const uint32_t as_addr = b_addr + L::kHalfBytes;
+          const uint32_t bs_addr = as_addr + S::kBytes;
+          // per scale tile: 4 columns for the tokens; 8 for the weight rows
+          const uint32_t as_col = tmem_base + L::kScaleCol + buf * L::kScaleBuf;
+          const uint32_t bs_col = as_col + 4 * S::kTiles;
+          const int steps = kblock_steps(g.K, kb);
+          for (int t = 0; t * S::kStepsPerTile < steps; ++t) {
+            tmem_copy_scale_tile<true>(as_col + 4 * t, make_desc_scale_tile(as_addr + 512 * t));
+            tmem_copy_scale_tile<true>(bs_col + 8 * t, make_desc_scale_tile(bs_addr + 512 * t));
+            tmem_copy_scale_tile<true>(bs_col + 8 * t + 4,
+                                       make_desc_scale_tile(bs_addr + S::kBytes + 512 * t));
+          }
+          for (int k = 0; k < steps; ++k) {
+            const int t = k / S::kStepsPerTile, id = k % S::kStepsPerTile * 2;
+            umma_fp4<true, S::kBlock>(d_tmem, make_desc_kmajor_sw128(a_addr + k * 32),
+                                      make_desc_kmajor_sw128(b_addr + k * 32),
+                                      make_idesc_fp4(kPairRows, kPairRows, S::kE8m0, id),
+                                      as_col + 4 * t, bs_col + 8 * t, (kb | k) != 0 ? 1u : 0u);
+          }
+          umma_commit_pair(&bar.empty[stage], 0x3);  // frees the stage in both CTAs
+          buf ^= 1u;
+          before = last;
+          before_phase = last_phase;
+          last = stage;
+          last_phase = phase;
+          if (++stage == kPairStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok) umma_commit_pair(bar.acc_full, 0x3);
+      }
+      if (!ok && last >= 0) mbar_wait_drain(&bar.empty[last], last_phase, g.status);
+    }
+    __syncwarp();
+  } else {
+    const uint32_t free_leader = map_to_cta(smem_u32(bar.acc_free), 0);
+    uint8_t* region = smem + L::kEpiOffset + (warp - 2) * kPairRegion;
+    const float* sb_s = reinterpret_cast<const float*>(region + kPairScaleCache);
+    const OutT* bias_s = reinterpret_cast<const OutT*>(region + kPairBiasCache);
+    const int q = warp & 3;
+    const int h = (warp - 2) >> 2;
+    const int row_in_tile = static_cast<int>(rank) * 128 + q * 32;
+    PairConsts next{};
+    if (pair < tiles) {
+      int mb, nb;
+      tile_coords(pair, g.num_m, g.num_n, mb, nb, 0, 0, g.group_n);
+      next = pair_consts<FORMAT, OutT>(g, nb, h, static_cast<int64_t>(mb) * kPairRows + row_in_tile + lane,
+                                       lane);
+    }
+    int i = 0;
+    for (int tile = pair; tile < tiles; tile += pairs, ++i) {
+      int mb, nb;
+      tile_coords(tile, g.num_m, g.num_n, mb, nb, 0, 0, g.group_n);
+      __syncwarp();
+      pair_consts_store<FORMAT, OutT>(region, next, lane);
+      const float sa = next.sa;
+      __syncwarp();
+      if (tile + pairs < tiles) {  // the next tile's constants, a tile ahead
+        int mb1, nb1;
+        tile_coords(tile + pairs, g.num_m, g.num_n, mb1, nb1, 0, 0, g.group_n);
+        next = pair_consts<FORMAT, OutT>(
+            g, nb1, h, static_cast<int64_t>(mb1) * kPairRows + row_in_tile + lane, lane);
+      }
+      if (!mbar_wait(bar.acc_full, i & 1, bar.abort_flag, g.status)) break;
+      tc_fence_after();
+      const int64_t row = static_cast<int64_t>(mb) * kPairRows + row_in_tile;
+      const uint32_t t_row =
+          tmem_base + (static_cast<uint32_t>(q * 32) << 16) + (i & 1) * L::kAccStep;
+#pragma unroll 1
+      for (int step = 0; step < 2; ++step) {
+        // the shared columns first: the upper half of accumulator 0, the lower of 1
+        const int piece = (i & 1) ? step : 1 - step;
+        const int in_tile = 128 * piece + 64 * h;
+        uint32_t r[2][32];
+        tmem_ld_32x32b_x32(t_row + in_tile, r[0]);
+        tmem_ld_32x32b_x32(t_row + in_tile + 32, r[1]);
+        tmem_ld_wait();
+        if (step == 0) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(free_leader);
+        }
+        const int col = nb * kPairRows + in_tile;
+        pair_scale32<FORMAT, OutT>(g, r[0], sa, sb_s + 64 * piece, bias_s + 64 * piece);
+        pair_scale32<FORMAT, OutT>(g, r[1], sa, sb_s + 64 * piece + 32, bias_s + 64 * piece + 32);
+        float y[32];
+        if (g.epilogue & TM_EPI_SWIGLU) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            y[j] = swiglu(__uint_as_float(r[j >> 4][j & 15]), __uint_as_float(r[j >> 4][16 + (j & 15)]));
+          pair_store32<OutT>(&tm_out, region, y, col / 2, row, row < g.M && col < g.N, lane);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) y[j] = activate(__uint_as_float(r[k][j]), g.epilogue);
+            pair_store32<OutT>(&tm_out, region, y, col + 32 * k, row,
+                               row < g.M && col + 32 * k < g.N, lane);
+          }
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_all();  // stores done before the CTA ends
+  }
+
+  tc_fence_before();
+  cluster_sync();  // no CTA leaves while its peer may still signal it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
 // ====================================================================== host
 struct Fp4Operand {
   const uint8_t* codes;
@@ -427,14 +801,89 @@ int launch_small(const Fp4Operand& x, const Fp4Operand& w, Fp4Args args, int spl
   return check_launch();
 }
 
+// Resident pairs of the pair kernel on a device (cached; both formats and
+// output types need the same resources per CTA but for a few KiB of shared memory).
+int max_fp4_pairs(int device, int sms) {
+  static int cache[64] = {};
+  if (device < 0 || device >= 64) return 0;
+  if (cache[device] == 0) {
+    auto kernel = gemm_fp4_pair_kernel<TM_FP4_NV, __nv_bfloat16>;
+    constexpr int smem = PairLayout<TM_FP4_NV>::kTotal;
+    int clusters = 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) ==
+        cudaSuccess) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(static_cast<unsigned>(sms & ~1));
+      cfg.blockDim = dim3(kPairThreads);
+      cfg.dynamicSmemBytes = smem;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 2;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) clusters = 0;
+    }
+    cudaGetLastError();  // a failed query must not poison later launches
+    cache[device] = clusters > 0 ? clusters : -1;
+  }
+  return cache[device] > 0 ? cache[device] : 0;
+}
+
+template <int FORMAT, typename OutT>
+int launch_pair_fp4(const Fp4Operand& x, const Fp4Operand& w, Fp4Args args, int max_pairs,
+                    cudaStream_t stream) {
+  using L = PairLayout<FORMAT>;
+  if (max_pairs <= 0) return TM_ERR_UNSUPPORTED;
+  args.num_m = (args.M + kPairRows - 1) / kPairRows;
+  args.num_n = (args.N + kPairRows - 1) / kPairRows;
+  args.group_n = choose_group_n(args.num_n, kPairRows, kPairRows, args.K / 2);
+  const int64_t tiles = static_cast<int64_t>(args.num_m) * args.num_n;
+  if (tiles > 0x3fffffffLL) return TM_ERR_TOO_LARGE;
+  const int64_t out_cols = (args.epilogue & TM_EPI_SWIGLU) ? args.N / 2 : args.N;
+  CUtensorMap ta, tb, tas, tbs, to;
+  if (!encode_codes(&ta, x, args.K, 128) || !encode_codes(&tb, w, args.K, 128) ||
+      !encode_scales<FORMAT>(&tas, x, args.K, 1) || !encode_scales<FORMAT>(&tbs, w, args.K, 2) ||
+      !encode_tmap_2d(&to,
+                      std::is_same<OutT, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                      args.out, out_cols, args.M, static_cast<uint64_t>(args.ldo) * 2, 32, 32,
+                      CU_TENSOR_MAP_SWIZZLE_64B))
+    return TM_ERR_CUDA;
+  auto kernel = gemm_fp4_pair_kernel<FORMAT, OutT>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal) !=
+      cudaSuccess)
+    return TM_ERR_CUDA;
+  const int pairs = static_cast<int>(tiles < max_pairs ? tiles : max_pairs);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = L::kTotal;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  if (launch_with_pdl(cfg, attr, 1, kernel, ta, tb, tas, tbs, to, args) != cudaSuccess)
+    return TM_ERR_CUDA;
+  return check_launch();
+}
+
 // Tile configurations: 32, 64, 128 = the small kernel with that many tokens a
-// tile (32 and 64 only for M up to that); 0 = chosen here.
+// tile (32 and 64 only for M up to that); kPairTile = the pair kernel; 0 =
+// chosen here.
+constexpr int kPairTile = 1256;
+
 struct Fp4Choice {
   int tile;
   int splits;
 };
 
-Fp4Choice pick_fp4(int64_t m, int64_t n, int kblocks, int sms) {
+Fp4Choice pick_fp4(int64_t m, int64_t n, int kblocks, int sms, int max_pairs) {
+  if (m > 128 && max_pairs > 0 && ((m + 255) / 256) * ((n + 255) / 256) * 2 >= max_pairs)
+    return Fp4Choice{kPairTile, 1};
   Fp4Choice c{m <= 32 ? 32 : m <= 64 ? 64 : 128, 1};
   const int64_t tiles = (m + c.tile - 1) / c.tile * ((n + kTileRows - 1) / kTileRows);
   while (c.splits < 8 && tiles * c.splits * 2 <= 2 * sms && kblocks >= 4 * c.splits) c.splits *= 2;
@@ -443,11 +892,12 @@ Fp4Choice pick_fp4(int64_t m, int64_t n, int kblocks, int sms) {
 
 template <int FORMAT, typename OutT>
 int dispatch_fp4(const Fp4Operand& x, const Fp4Operand& w, const Fp4Args& args, Fp4Choice c,
-                 cudaStream_t stream) {
+                 int max_pairs, cudaStream_t stream) {
   switch (c.tile) {
     case 32: return launch_small<32, FORMAT, OutT>(x, w, args, c.splits, stream);
     case 64: return launch_small<64, FORMAT, OutT>(x, w, args, c.splits, stream);
     case 128: return launch_small<128, FORMAT, OutT>(x, w, args, c.splits, stream);
+    case kPairTile: return launch_pair_fp4<FORMAT, OutT>(x, w, args, max_pairs, stream);
     default: return TM_ERR_UNSUPPORTED;
   }
 }
@@ -492,21 +942,22 @@ int scaled_mm_fp4_impl(void* out, int out_dtype, const uint8_t* a, const uint8_t
   args.kblocks = static_cast<int>((k + kKBlock - 1) / kKBlock);
   args.epilogue = epilogue;
   args.status = device_status_ptr(device);
+  const int max_pairs = max_fp4_pairs(device, sms);
   Fp4Choice c{tile, splits};
   if (tile == 0) {
-    c = pick_fp4(m, n, args.kblocks, sms);
+    c = pick_fp4(m, n, args.kblocks, sms, max_pairs);
   } else {
     if (splits != 1 && splits != 2 && splits != 4 && splits != 8) return TM_ERR_UNSUPPORTED;
-    if (tile < 128 && m > tile) return TM_ERR_UNSUPPORTED;
+    if ((tile < 128 && m > tile) || (tile == kPairTile && splits != 1)) return TM_ERR_UNSUPPORTED;
   }
   const Fp4Operand x{a, lda, blocks_a, m}, w{b, ldb, blocks_b, n};
   const cudaStream_t st = as_stream(stream);
   const bool bf16 = out_dtype == TM_DTYPE_BF16;
   if (format == TM_FP4_NV)
-    return bf16 ? dispatch_fp4<TM_FP4_NV, __nv_bfloat16>(x, w, args, c, st)
-                : dispatch_fp4<TM_FP4_NV, __half>(x, w, args, c, st);
-  return bf16 ? dispatch_fp4<TM_FP4_MX, __nv_bfloat16>(x, w, args, c, st)
-              : dispatch_fp4<TM_FP4_MX, __half>(x, w, args, c, st);
+    return bf16 ? dispatch_fp4<TM_FP4_NV, __nv_bfloat16>(x, w, args, c, max_pairs, st)
+                : dispatch_fp4<TM_FP4_NV, __half>(x, w, args, c, max_pairs, st);
+  return bf16 ? dispatch_fp4<TM_FP4_MX, __nv_bfloat16>(x, w, args, c, max_pairs, st)
+              : dispatch_fp4<TM_FP4_MX, __half>(x, w, args, c, max_pairs, st);
 }
 
 }  // namespace

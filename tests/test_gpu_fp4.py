@@ -283,3 +283,19 @@ def test_mm_epilogues(tm_ops, cuda, m, n, k, act, fmt):
         out = tm_ops.scaled_mm_fp4(aq, wq.t(), ab, wb, asc, wsc, bias=b, gelu_tanh=act == "gelu",
                                    swiglu=act == "swiglu")
         _check_mm(out, *ops, b, fmt, act)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("act,dtype", [("none", torch.bfloat16), ("gelu", torch.float16),
+                                       ("swiglu", torch.bfloat16)])
+@pytest.mark.parametrize("m,n,k", [(1, 64, 32), (256, 256, 256), (129, 448, 96), (300, 1344, 800),
+                                   (517, 2112, 1376), (2049, 5120, 544), (5000, 4160, 288)])
+def test_mm_pair_tile(tm_ops, cuda, m, n, k, act, dtype, fmt):
+    """The CTA-pair kernel: one tile to several waves, tails in every dimension."""
+    *ops, bias = _operands(tm_ops, cuda, m, n, k, fmt, dtype, m + n + k)
+    aq, ab, asc, wq, wb, wsc = ops
+    out = tm_ops.scaled_mm_fp4(aq, wq.t(), ab, wb, asc, wsc, dtype, bias, gelu_tanh=act == "gelu",
+                               swiglu=act == "swiglu", tile=1256)
+    _check_mm(out, *ops, bias, fmt, act)
+    plain = tm_ops.scaled_mm_fp4(aq, wq.t(), ab, wb, asc, wsc, dtype, tile=1256)
+    _check_mm(plain, *ops, None, fmt)
