@@ -594,7 +594,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (leader && lane == 0) {
+    // The whole warp runs the loop; one elected lane issues (see elect_one).
+    if (leader) {
+      const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
       int stage = 0;
       uint32_t phase = 0;
       int last = -1, before = -1;  // stages of the previous k-block and of the one before it
@@ -610,7 +612,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           break;
         }
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + (i & 1) * L::kAccStep;
+        const uint32_t d_tmem = tmem + (i & 1) * L::kAccStep;
         for (int kb = 0; kb < g.kblocks; ++kb) {
           // the scale buffer was last read two k-blocks ago
           if ((before >= 0 &&
@@ -620,28 +622,37 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             break;
           }
           tc_fence_after();
-          const uint32_t a_addr = smem_u32(smem + stage * L::kStageBytes);
-          const uint32_t b_addr = a_addr + L::kHalfBytes;
-          const uint32_t as_addr = b_addr + L::kHalfBytes;
-          const uint32_t bs_addr = as_addr + S::kBytes;
+          __syncwarp();
+          const uint32_t a_addr = smem_u32(smem) + stage * L::kStageBytes;
+          const uint64_t a_desc = make_desc_kmajor_sw128(a_addr);
+          const uint64_t b_desc = make_desc_kmajor_sw128(a_addr + L::kHalfBytes);
+          const uint64_t as_desc = make_desc_scale_tile(a_addr + 2 * L::kHalfBytes);
+          const uint64_t bs_desc = make_desc_scale_tile(a_addr + 2 * L::kHalfBytes + S::kBytes);
           // per scale tile: 4 columns for the tokens; 8 for the weight rows
-          const uint32_t as_col = tmem_base + L::kScaleCol + buf * L::kScaleBuf;
+          const uint32_t as_col = tmem + L::kScaleCol + buf * L::kScaleBuf;
           const uint32_t bs_col = as_col + 4 * S::kTiles;
           const int steps = kblock_steps(g.K, kb);
-          for (int t = 0; t * S::kStepsPerTile < steps; ++t) {
-            tmem_copy_scale_tile<true>(as_col + 4 * t, make_desc_scale_tile(as_addr + 512 * t));
-            tmem_copy_scale_tile<true>(bs_col + 8 * t, make_desc_scale_tile(bs_addr + 512 * t));
-            tmem_copy_scale_tile<true>(bs_col + 8 * t + 4,
-                                       make_desc_scale_tile(bs_addr + S::kBytes + 512 * t));
+          if (elect_one()) {
+            // descriptors count 16-byte units
+#pragma unroll
+            for (int t = 0; t < S::kTiles; ++t) {
+              if (t * S::kStepsPerTile < steps) {
+                tmem_copy_scale_tile<true>(as_col + 4 * t, as_desc + 32 * t);
+                tmem_copy_scale_tile<true>(bs_col + 8 * t, bs_desc + 32 * t);
+                tmem_copy_scale_tile<true>(bs_col + 8 * t + 4, bs_desc + S::kBytes / 16 + 32 * t);
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < kKBlock / kMmaK; ++k) {
+              const int t = k / S::kStepsPerTile, id = k % S::kStepsPerTile * 2;
+              if (k < steps)
+                umma_fp4<true, S::kBlock>(d_tmem, a_desc + 2 * k, b_desc + 2 * k,
+                                          make_idesc_fp4(kPairRows, kPairRows, S::kE8m0, id),
+                                          as_col + 4 * t, bs_col + 8 * t, (kb | k) != 0 ? 1u : 0u);
+            }
+            umma_commit_pair(&bar.empty[stage], 0x3);  // frees the stage in both CTAs
           }
-          for (int k = 0; k < steps; ++k) {
-            const int t = k / S::kStepsPerTile, id = k % S::kStepsPerTile * 2;
-            umma_fp4<true, S::kBlock>(d_tmem, make_desc_kmajor_sw128(a_addr + k * 32),
-                                      make_desc_kmajor_sw128(b_addr + k * 32),
-                                      make_idesc_fp4(kPairRows, kPairRows, S::kE8m0, id),
-                                      as_col + 4 * t, bs_col + 8 * t, (kb | k) != 0 ? 1u : 0u);
-          }
-          umma_commit_pair(&bar.empty[stage], 0x3);  // frees the stage in both CTAs
+          __syncwarp();
           buf ^= 1u;
           before = last;
           before_phase = last_phase;
@@ -652,7 +663,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             phase ^= 1u;
           }
         }
-        if (ok) umma_commit_pair(bar.acc_full, 0x3);
+        if (ok && elect_one()) umma_commit_pair(bar.acc_full, 0x3);
+        __syncwarp();
       }
       if (!ok && last >= 0) mbar_wait_drain(&bar.empty[last], last_phase, g.status);
     }
