@@ -10,16 +10,15 @@
 // A k-block is 128 bytes (256 elements) of K: one swizzle row of codes, four
 // MMAs of K = 64.  Its scales are 4 (TM_FP4_NV) or 2 (TM_FP4_MX) 512-byte tiles
 // for each 128 rows; they travel by TMA beside the codes and are copied to TMEM
-// by the MMA thread (tcgen05.cp, in order with its MMAs).  Two TMEM scale
-// buffers alternate; one is written again only after the MMAs that read it
-// have completed.
+// by the MMA thread (tcgen05.cp, in order with its MMAs); the columns of a scale
+// tile are written again only after the MMAs that read them have completed.
 //
 //   gemm_fp4_pair_kernel  persistent CTA pairs (clusters of 2), a 256 token x 256
 //     weight row tile each: a CTA fetches 128 token rows and 128 weight rows, the
 //     leader issues tcgen05.mma.cta_group::2 (M = 256, N = 256), and each CTA's
 //     TMEM receives 128 x 256 sums.  Two such accumulators and the scales exceed
-//     the 512 TMEM columns, so the accumulators overlap by 128: an epilogue first
-//     takes the shared columns into registers, then lets the next tile start.
+//     the 512 TMEM columns, so there is one: the epilogue takes it into registers
+//     (128 columns a warp) and converts and stores while the next tile runs.
 //   gemm_fp4_small_kernel  one CTA per (128 weight rows x TOK tokens, K slice).
 //     The weight is the M operand (128 TMEM lanes), the tokens the N operand, so
 //     one token costs a 32-column accumulator and the weight streams once.
@@ -56,6 +55,7 @@ struct Fp4Args {
   int num_m, num_n;
   int group_n;
   int stages;
+  bool wide;  // output rows start on 32-byte boundaries
   uint32_t epilogue;
   int* status;
 };
@@ -373,10 +373,15 @@ constexpr int kPairThreads = 320;  // producer, MMA, eight epilogue warps
 constexpr int kPairEpiWarps = 8;
 constexpr int kPairRows = 256;     // tokens, and weight rows, of a tile
 constexpr int kPairStages = 5;
-// per epilogue warp: a staging tile, 128 column scales and 128 bias values
-constexpr int kPairScaleCache = kStage64Bytes;
-constexpr int kPairBiasCache = kPairScaleCache + 512;
-constexpr int kPairRegion = 4096;
+// per epilogue warp: 128 column scales and 128 bias values
+constexpr int kPairBiasCache = 512;
+constexpr int kPairRegion = 768;
+// TMEM: the 256-column accumulator, then each stage's scale tiles (4 columns
+// for the tokens and 8 for the weight rows): a stage's columns are written
+// again when its shared memory has been refilled, hence after its MMAs.
+constexpr uint32_t kScaleCol = 256;
+constexpr int kTileCols = 12;
+static_assert(kScaleCol + kPairStages * 4 * kTileCols <= 512, "TMEM columns");
 
 template <int FORMAT>
 struct PairLayout {
@@ -384,15 +389,10 @@ struct PairLayout {
   static constexpr int kHalfBytes = 128 * kRowBytes;
   static constexpr int kStageBytes = 2 * kHalfBytes + 3 * S::kBytes;  // per CTA
   static constexpr int kBarOffset = kPairStages * kStageBytes;
-  static constexpr int kEpiOffset = (kBarOffset + 256 + 1023) / 1024 * 1024;
+  static constexpr int kEpiOffset = kBarOffset + 256;
   static constexpr int kTotal = kEpiOffset + kPairEpiWarps * kPairRegion + 1024;
   static_assert(kStageBytes % 1024 == 0, "stages stay aligned");
   static_assert(kTotal <= 227 * 1024, "shared memory budget");
-  // TMEM: accumulator b at columns [128 b, 128 b + 256), scale buffers behind
-  static constexpr uint32_t kAccStep = 128;
-  static constexpr uint32_t kScaleCol = 384;
-  static constexpr uint32_t kScaleBuf = 3 * 4 * S::kTiles;
-  static_assert(kScaleCol + 2 * kScaleBuf <= 512, "TMEM columns");
 };
 
 struct PairBars {
@@ -415,8 +415,8 @@ __device__ __forceinline__ PairBars pair_bars(uint8_t* base) {
   return b;
 }
 
-// A lane's share of a tile's constants: four columns' scales and bias values
-// and its row's scale.  Columns of piece p (lane / 16): 128 p + 64 h + 4 (lane % 16).
+// A lane's share of a tile's constants: the scales and bias values of four of
+// the warp's 128 columns, and its row's scale.
 struct PairConsts {
   float sb[4];
   float bias[4];
@@ -427,7 +427,7 @@ template <int FORMAT, typename OutT>
 __device__ __forceinline__ PairConsts pair_consts(const Fp4Args& g, int nb, int h, int64_t row,
                                                   int lane) {
   PairConsts c;
-  const int col = nb * kPairRows + 128 * (lane >> 4) + 64 * h + 4 * (lane & 15);
+  const int col = nb * kPairRows + 128 * h + 4 * lane;
   const bool in = col < g.N;  // N % 8 == 0: all four or none
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -442,7 +442,7 @@ __device__ __forceinline__ PairConsts pair_consts(const Fp4Args& g, int nb, int 
 template <int FORMAT, typename OutT>
 __device__ __forceinline__ void pair_consts_store(uint8_t* region, const PairConsts& c, int lane) {
   if constexpr (FORMAT == TM_FP4_NV)
-    *reinterpret_cast<float4*>(region + kPairScaleCache + 16 * lane) =
+    *reinterpret_cast<float4*>(region + 16 * lane) =
         make_float4(c.sb[0], c.sb[1], c.sb[2], c.sb[3]);
   *reinterpret_cast<uint2*>(region + kPairBiasCache + 8 * lane) =
       make_uint2(pack2<OutT>(c.bias[0], c.bias[1]), pack2<OutT>(c.bias[2], c.bias[3]));
@@ -478,23 +478,29 @@ __device__ __forceinline__ void pair_scale32(const Fp4Args& g, uint32_t (&r)[32]
   }
 }
 
-// Stage 32 rows x 32 columns (a row per lane) and store them by TMA.
+// Store 32 columns of this lane's row, full 32-byte sectors where the output
+// allows it (`wide`: rows start on 32-byte boundaries).  Straight from
+// registers: staged TMA stores wait in the queue of the operand loads, and the
+// epilogue with them (8192 x 12288 x 3072 nvfp4: WIDE_FIGURE).
 template <typename OutT>
-__device__ __forceinline__ void pair_store32(const CUtensorMap* tm_out, uint8_t* region,
-                                             const float (&y)[32], int x, int64_t row, bool in,
-                                             int lane) {
-  if (lane == 0) bulk_wait_read_all();  // the previous store has left the tile
-  __syncwarp();
+__device__ __forceinline__ void pair_store32(OutT* row, const float (&y)[32], int col, int cols,
+                                             bool wide) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    *stage64_slot(region, lane, j) =
-        make_uint4(pack2<OutT>(y[8 * j], y[8 * j + 1]), pack2<OutT>(y[8 * j + 2], y[8 * j + 3]),
-                   pack2<OutT>(y[8 * j + 4], y[8 * j + 5]), pack2<OutT>(y[8 * j + 6], y[8 * j + 7]));
-  fence_async_shared();
-  __syncwarp();
-  if (lane == 0 && in) {
-    tma_store_2d(tm_out, region, x, static_cast<int>(row));
-    bulk_commit();
+  for (int j = 0; j < 32; j += 16) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = pack2<OutT>(y[j + 2 * i], y[j + 2 * i + 1]);
+    OutT* dst = row + col + j;
+    if (wide && col + j + 16 <= cols) {
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(w[0]),
+                   "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                   : "memory");
+    } else {  // columns come in multiples of 8
+      if (col + j + 8 <= cols)
+        *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (col + j + 16 <= cols)
+        *reinterpret_cast<uint4*>(dst + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+    }
   }
 }
 
@@ -503,8 +509,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
                          const __grid_constant__ CUtensorMap tm_b,
                          const __grid_constant__ CUtensorMap tm_as,
-                         const __grid_constant__ CUtensorMap tm_bs,
-                         const __grid_constant__ CUtensorMap tm_out, const Fp4Args g) {
+                         const __grid_constant__ CUtensorMap tm_bs, const Fp4Args g) {
   using L = PairLayout<FORMAT>;
   using S = ScaleGeom<FORMAT>;
   extern __shared__ uint8_t smem_raw[];
@@ -513,7 +518,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_ctarank();  // 0 = leader (issues the MMAs)
+  const uint32_t rank = blockIdx.x & 1;  // in the cluster of 2; 0 = leader (issues the MMAs)
   const bool leader = rank == 0;
   const int tiles = g.num_m * g.num_n;
   const int pair = blockIdx.x >> 1;
@@ -532,7 +537,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     tma_prefetch_desc(&tm_b);
     tma_prefetch_desc(&tm_as);
     tma_prefetch_desc(&tm_bs);
-    tma_prefetch_desc(&tm_out);
   }
   if (warp == 1) {
     tmem_alloc_pair(bar.tmem_slot, 512);
@@ -546,39 +550,44 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   griddep_launch_dependents();
 
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      uint32_t issued_mask = 0, issued_parity = 0;
-      bool ok = true;
-      for (int tile = pair; ok && tile < tiles; tile += pairs) {
-        int mb, nb;
-        tile_coords(tile, g.num_m, g.num_n, mb, nb, 0, 0, g.group_n);
-        for (int kb = 0; kb < g.kblocks; ++kb) {
-          if (!mbar_wait(&bar.empty[stage], phase ^ 1u, bar.abort_flag, g.status)) {
-            ok = false;
-            break;
-          }
-          issued_mask &= ~(1u << stage);
+    int stage = 0;
+    uint32_t phase = 0;
+    uint32_t issued_mask = 0, issued_parity = 0;
+    bool ok = true;
+    for (int tile = pair; ok && tile < tiles; tile += pairs) {
+      int mb, nb;
+      tile_coords(tile, g.num_m, g.num_n, mb, nb, 0, 0, g.group_n);
+      for (int kb = 0; kb < g.kblocks; ++kb) {
+        if (!mbar_wait_warp(&bar.empty[stage], phase ^ 1u, bar.abort_flag, g.status)) {
+          ok = false;
+          break;
+        }
+        issued_mask &= ~(1u << stage);
+        if (elect_one()) {
           uint8_t* s = smem + stage * L::kStageBytes;
           uint8_t* scales = s + 2 * L::kHalfBytes;
           // the leader's `full` barrier counts the bytes landing in both CTAs
           if (leader) mbar_arrive_expect_tx(&bar.full[stage], 2 * L::kStageBytes);
           const uint32_t full = map_to_cta(smem_u32(&bar.full[stage]), 0);
-          tma_load_2d_pair(&tm_a, full, s, kb * kRowBytes, mb * kPairRows + static_cast<int>(rank) * 128);
+          tma_load_2d_pair(&tm_a, full, s, kb * kRowBytes,
+                           mb * kPairRows + static_cast<int>(rank) * 128);
           tma_load_2d_pair(&tm_b, full, s + L::kHalfBytes, kb * kRowBytes,
                            nb * kPairRows + static_cast<int>(rank) * 128);
           // own tokens' scales, and the whole tile's weight scales in both CTAs
-          tma_load_2d_pair(&tm_as, full, scales, kb * (S::kBytes / 8), mb * 2 + static_cast<int>(rank));
+          tma_load_2d_pair(&tm_as, full, scales, kb * (S::kBytes / 8),
+                           mb * 2 + static_cast<int>(rank));
           tma_load_2d_pair(&tm_bs, full, scales + S::kBytes, kb * (S::kBytes / 8), nb * 2);
-          issued_mask |= 1u << stage;
-          issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
-          if (++stage == kPairStages) {
-            stage = 0;
-            phase ^= 1u;
-          }
+        }
+        __syncwarp();
+        issued_mask |= 1u << stage;
+        issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
+        if (++stage == kPairStages) {
+          stage = 0;
+          phase ^= 1u;
         }
       }
+    }
+    if (lane == 0) {
       if (!ok) {
         if (leader) {
           for (int s = 0; s < kPairStages; ++s)
@@ -594,70 +603,65 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    // The whole warp runs the loop; one elected lane issues (see elect_one).
+    // the whole warp runs the loop, one lane issues (see elect_one)
     if (leader) {
-      const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+      const uint32_t tmem = __reduce_max_sync(0xffffffffu, tmem_base);
+      const uint32_t smem0 = smem_u32(smem);
       int stage = 0;
       uint32_t phase = 0;
-      int last = -1, before = -1;  // stages of the previous k-block and of the one before it
-      uint32_t last_phase = 0, before_phase = 0;
-      uint32_t buf = 0;  // scale buffer
-      bool ok = true;
+      bool ok = true, issued_any = false;
       int i = 0;
       for (int tile = pair; ok && tile < tiles; tile += pairs, ++i) {
-        // the previous tile's epilogue holds the columns the accumulators share
-        // (and has finished with everything before)
-        if (i > 0 && !mbar_wait(bar.acc_free, (i - 1) & 1, bar.abort_flag, g.status)) {
+        // the previous tile's sums are in the epilogue's registers
+        if (i > 0 && !mbar_wait_warp(bar.acc_free, (i - 1) & 1, bar.abort_flag, g.status)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t d_tmem = tmem + (i & 1) * L::kAccStep;
         for (int kb = 0; kb < g.kblocks; ++kb) {
-          // the scale buffer was last read two k-blocks ago
-          if ((before >= 0 &&
-               !mbar_wait(&bar.empty[before], before_phase, bar.abort_flag, g.status)) ||
-              !mbar_wait(&bar.full[stage], phase, bar.abort_flag, g.status)) {
+          if (!mbar_wait_warp(&bar.full[stage], phase, bar.abort_flag, g.status)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          __syncwarp();
-          const uint32_t a_addr = smem_u32(smem) + stage * L::kStageBytes;
-          const uint64_t a_desc = make_desc_kmajor_sw128(a_addr);
-          const uint64_t b_desc = make_desc_kmajor_sw128(a_addr + L::kHalfBytes);
-          const uint64_t as_desc = make_desc_scale_tile(a_addr + 2 * L::kHalfBytes);
-          const uint64_t bs_desc = make_desc_scale_tile(a_addr + 2 * L::kHalfBytes + S::kBytes);
-          // per scale tile: 4 columns for the tokens; 8 for the weight rows
-          const uint32_t as_col = tmem + L::kScaleCol + buf * L::kScaleBuf;
-          const uint32_t bs_col = as_col + 4 * S::kTiles;
+          const uint32_t base = smem0 + stage * L::kStageBytes;
+          const uint64_t a_desc = make_desc_kmajor_sw128(base);
+          const uint64_t b_desc = make_desc_kmajor_sw128(base + L::kHalfBytes);
+          const uint64_t as_desc = make_desc_scale_tile(base + 2 * L::kHalfBytes);
+          const uint64_t bs_desc = make_desc_scale_tile(base + 2 * L::kHalfBytes + S::kBytes);
+          const uint32_t col = tmem + kScaleCol + stage * (S::kTiles * kTileCols);
+          const uint32_t more = kb != 0 ? 1u : 0u;
           const int steps = kblock_steps(g.K, kb);
-          if (elect_one()) {
-            // descriptors count 16-byte units
+          // descriptors count 16-byte units
+          const auto copy = [&](int t) {
+            tmem_copy_scale_tile<true>(col + kTileCols * t, as_desc + 32 * t);
+            tmem_copy_scale_tile<true>(col + kTileCols * t + 4, bs_desc + 32 * t);
+            tmem_copy_scale_tile<true>(col + kTileCols * t + 8, bs_desc + S::kBytes / 16 + 32 * t);
+          };
+          const auto multiply = [&](int k) {
+            const int t = k / S::kStepsPerTile;
+            umma_fp4<true, S::kBlock>(
+                tmem, a_desc + 2 * k, b_desc + 2 * k,
+                make_idesc_fp4(kPairRows, kPairRows, S::kE8m0, k % S::kStepsPerTile * 2),
+                col + kTileCols * t, col + kTileCols * t + 4, k == 0 ? more : 1u);
+          };
+          if (steps == kKBlock / kMmaK) {
+            if (elect_one()) {
 #pragma unroll
-            for (int t = 0; t < S::kTiles; ++t) {
-              if (t * S::kStepsPerTile < steps) {
-                tmem_copy_scale_tile<true>(as_col + 4 * t, as_desc + 32 * t);
-                tmem_copy_scale_tile<true>(bs_col + 8 * t, bs_desc + 32 * t);
-                tmem_copy_scale_tile<true>(bs_col + 8 * t + 4, bs_desc + S::kBytes / 16 + 32 * t);
-              }
-            }
+              for (int t = 0; t < S::kTiles; ++t) copy(t);
 #pragma unroll
-            for (int k = 0; k < kKBlock / kMmaK; ++k) {
-              const int t = k / S::kStepsPerTile, id = k % S::kStepsPerTile * 2;
-              if (k < steps)
-                umma_fp4<true, S::kBlock>(d_tmem, a_desc + 2 * k, b_desc + 2 * k,
-                                          make_idesc_fp4(kPairRows, kPairRows, S::kE8m0, id),
-                                          as_col + 4 * t, bs_col + 8 * t, (kb | k) != 0 ? 1u : 0u);
+              for (int k = 0; k < kKBlock / kMmaK; ++k) multiply(k);
+              umma_commit_pair(&bar.empty[stage], 0x3);  // frees the stage in both CTAs
             }
-            umma_commit_pair(&bar.empty[stage], 0x3);  // frees the stage in both CTAs
+          } else {  // the last k-block of a K that is not a multiple of 256
+            if (elect_one()) {
+              for (int t = 0; t * S::kStepsPerTile < steps; ++t) copy(t);
+              for (int k = 0; k < steps; ++k) multiply(k);
+              umma_commit_pair(&bar.empty[stage], 0x3);
+            }
           }
           __syncwarp();
-          buf ^= 1u;
-          before = last;
-          before_phase = last_phase;
-          last = stage;
-          last_phase = phase;
+          issued_any = true;
           if (++stage == kPairStages) {
             stage = 0;
             phase ^= 1u;
@@ -666,13 +670,16 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         if (ok && elect_one()) umma_commit_pair(bar.acc_full, 0x3);
         __syncwarp();
       }
-      if (!ok && last >= 0) mbar_wait_drain(&bar.empty[last], last_phase, g.status);
+      if (!ok && issued_any) {  // the last commit: the tensor pipe has drained
+        const int last = stage == 0 ? kPairStages - 1 : stage - 1;
+        mbar_wait_drain(&bar.empty[last], stage == 0 ? (phase ^ 1u) : phase, g.status);
+      }
     }
     __syncwarp();
   } else {
     const uint32_t free_leader = map_to_cta(smem_u32(bar.acc_free), 0);
     uint8_t* region = smem + L::kEpiOffset + (warp - 2) * kPairRegion;
-    const float* sb_s = reinterpret_cast<const float*>(region + kPairScaleCache);
+    const float* sb_s = reinterpret_cast<const float*>(region);
     const OutT* bias_s = reinterpret_cast<const OutT*>(region + kPairBiasCache);
     const int q = warp & 3;
     const int h = (warp - 2) >> 2;
@@ -700,44 +707,40 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
       if (!mbar_wait(bar.acc_full, i & 1, bar.abort_flag, g.status)) break;
       tc_fence_after();
-      const int64_t row = static_cast<int64_t>(mb) * kPairRows + row_in_tile;
-      const uint32_t t_row =
-          tmem_base + (static_cast<uint32_t>(q * 32) << 16) + (i & 1) * L::kAccStep;
-#pragma unroll 1
-      for (int step = 0; step < 2; ++step) {
-        // the shared columns first: the upper half of accumulator 0, the lower of 1
-        const int piece = (i & 1) ? step : 1 - step;
-        const int in_tile = 128 * piece + 64 * h;
-        uint32_t r[2][32];
-        tmem_ld_32x32b_x32(t_row + in_tile, r[0]);
-        tmem_ld_32x32b_x32(t_row + in_tile + 32, r[1]);
-        tmem_ld_wait();
-        if (step == 0) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(free_leader);
-        }
-        const int col = nb * kPairRows + in_tile;
-        pair_scale32<FORMAT, OutT>(g, r[0], sa, sb_s + 64 * piece, bias_s + 64 * piece);
-        pair_scale32<FORMAT, OutT>(g, r[1], sa, sb_s + 64 * piece + 32, bias_s + 64 * piece + 32);
-        float y[32];
-        if (g.epilogue & TM_EPI_SWIGLU) {
+      const int64_t row = static_cast<int64_t>(mb) * kPairRows + row_in_tile + lane;
+      OutT* out_row = static_cast<OutT*>(g.out) + row * g.ldo;
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+      // the warp's 128 columns, then the accumulator belongs to the next tile
+      uint32_t r[4][32];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) tmem_ld_32x32b_x32(t_row + 128 * h + 32 * k, r[k]);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(free_leader);
+      const int col0 = nb * kPairRows + 128 * h;
+      float y[32];
+      if (g.epilogue & TM_EPI_SWIGLU) {
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+          pair_scale32<FORMAT, OutT>(g, r[k], sa, sb_s + 32 * k, bias_s + 32 * k);
+          pair_scale32<FORMAT, OutT>(g, r[k + 1], sa, sb_s + 32 * k + 32, bias_s + 32 * k + 32);
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            y[j] = swiglu(__uint_as_float(r[j >> 4][j & 15]), __uint_as_float(r[j >> 4][16 + (j & 15)]));
-          pair_store32<OutT>(&tm_out, region, y, col / 2, row, row < g.M && col < g.N, lane);
-        } else {
+            y[j] = swiglu(__uint_as_float(r[k + (j >> 4)][j & 15]),
+                          __uint_as_float(r[k + (j >> 4)][16 + (j & 15)]));
+          if (row < g.M) pair_store32<OutT>(out_row, y, (col0 + 32 * k) / 2, g.N / 2, g.wide);
+        }
+      } else {
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < 4; ++k) {
+          pair_scale32<FORMAT, OutT>(g, r[k], sa, sb_s + 32 * k, bias_s + 32 * k);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) y[j] = activate(__uint_as_float(r[k][j]), g.epilogue);
-            pair_store32<OutT>(&tm_out, region, y, col + 32 * k, row,
-                               row < g.M && col + 32 * k < g.N, lane);
-          }
+          for (int j = 0; j < 32; ++j) y[j] = activate(__uint_as_float(r[k][j]), g.epilogue);
+          if (row < g.M) pair_store32<OutT>(out_row, y, col0 + 32 * k, g.N, g.wide);
         }
       }
     }
-    if (lane == 0) bulk_wait_all();  // stores done before the CTA ends
   }
 
   tc_fence_before();
@@ -853,15 +856,10 @@ int launch_pair_fp4(const Fp4Operand& x, const Fp4Operand& w, Fp4Args args, int 
   args.group_n = choose_group_n(args.num_n, kPairRows, kPairRows, args.K / 2);
   const int64_t tiles = static_cast<int64_t>(args.num_m) * args.num_n;
   if (tiles > 0x3fffffffLL) return TM_ERR_TOO_LARGE;
-  const int64_t out_cols = (args.epilogue & TM_EPI_SWIGLU) ? args.N / 2 : args.N;
-  CUtensorMap ta, tb, tas, tbs, to;
+  args.wide = reinterpret_cast<uintptr_t>(args.out) % 32 == 0 && args.ldo % 16 == 0;
+  CUtensorMap ta, tb, tas, tbs;
   if (!encode_codes(&ta, x, args.K, 128) || !encode_codes(&tb, w, args.K, 128) ||
-      !encode_scales<FORMAT>(&tas, x, args.K, 1) || !encode_scales<FORMAT>(&tbs, w, args.K, 2) ||
-      !encode_tmap_2d(&to,
-                      std::is_same<OutT, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                      args.out, out_cols, args.M, static_cast<uint64_t>(args.ldo) * 2, 32, 32,
-                      CU_TENSOR_MAP_SWIZZLE_64B))
+      !encode_scales<FORMAT>(&tas, x, args.K, 1) || !encode_scales<FORMAT>(&tbs, w, args.K, 2))
     return TM_ERR_CUDA;
   auto kernel = gemm_fp4_pair_kernel<FORMAT, OutT>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal) !=
@@ -878,7 +876,7 @@ int launch_pair_fp4(const Fp4Operand& x, const Fp4Operand& w, Fp4Args args, int 
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  if (launch_with_pdl(cfg, attr, 1, kernel, ta, tb, tas, tbs, to, args) != cudaSuccess)
+  if (launch_with_pdl(cfg, attr, 1, kernel, ta, tb, tas, tbs, args) != cudaSuccess)
     return TM_ERR_CUDA;
   return check_launch();
 }

@@ -186,18 +186,26 @@ __device__ __forceinline__ void fence_async_shared() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-// One lane of a converged warp (all 32 lanes call).  Code that the whole warp
-// runs, with only the asynchronous instructions inside `if (elect_one())`,
-// keeps their operands in uniform registers; behind `lane == 0` every operand
-// of every tcgen05 instruction is moved there one by one.
+// True on one lane of a converged warp (all 32 lanes call).  Code that the
+// whole warp runs, with the asynchronous instructions alone in a straight
+// `if (elect_one())` block, keeps their operands in uniform registers; behind
+// `lane == 0`, with conditions inside the block, or predicated lane by lane,
+// each operand is moved there separately (measured: up to 60 cycles for each
+// tcgen05 instruction instead of 30, twice the time of the whole product).
 __device__ __forceinline__ bool elect_one() {
-  uint32_t ok;
+  uint32_t on;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "elect.sync _|p, 0xffffffff;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok));
-  return ok != 0;
+      : "=r"(on));
+  return on != 0;
+}
+
+// mbar_wait by a converged warp, one answer for all of it.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort,
+                                               int* status) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, status));
 }
 
 // ---------------------------------------------------------------- tcgen05
