@@ -448,63 +448,80 @@ __device__ __forceinline__ void pair_consts_store(uint8_t* region, const PairCon
       make_uint2(pack2<OutT>(c.bias[0], c.bias[1]), pack2<OutT>(c.bias[2], c.bias[3]));
 }
 
-// Outer scales and bias on 32 accumulator columns (in place).
-template <int FORMAT, typename OutT>
-__device__ __forceinline__ void pair_scale32(const Fp4Args& g, uint32_t (&r)[32], float sa,
-                                             const float* sb, const OutT* bias) {
+// gelu_tanh on two values.
+__device__ __forceinline__ uint64_t gelu_f32x2(uint64_t x) {
+  const uint64_t beta = f32x2(0.7978845608028654f, 0.7978845608028654f);
+  const uint64_t beta_kappa = f32x2(0.035677408136300125f, 0.035677408136300125f);
+  const uint64_t half = f32x2(0.5f, 0.5f);
+  const uint64_t inner = mul_f32x2(x, fma_f32x2(beta_kappa, mul_f32x2(x, x), beta));
+  const uint64_t h = mul_f32x2(half, x);
+  float a, b;
+  f32x2_split(inner, a, b);
+  return fma_f32x2(h, f32x2(tanh_approx(a), tanh_approx(b)), h);
+}
+
+// Outer scales, bias and (GELU) activation on 16 accumulator columns, in place.
+template <int FORMAT, int EPI, typename OutT>
+__device__ __forceinline__ void pair_finish16(uint32_t* r, uint64_t sa2, bool has_bias,
+                                              const float* sb, const OutT* bias) {
 #pragma unroll
-  for (int j = 0; j < 32; j += 8) {
-    float y[8];
+  for (int j = 0; j < 16; j += 4) {
+    uint64_t y[2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(r[j + i]);
+    for (int i = 0; i < 2; ++i)
+      y[i] = f32x2(__uint_as_float(r[j + 2 * i]), __uint_as_float(r[j + 2 * i + 1]));
     if constexpr (FORMAT == TM_FP4_NV) {
-      const float4 s0 = *reinterpret_cast<const float4*>(sb + j);
-      const float4 s1 = *reinterpret_cast<const float4*>(sb + j + 4);
-      const float sc[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(sc[i], y[i]);
+      const float4 s = *reinterpret_cast<const float4*>(sb + j);
+      y[0] = mul_f32x2(y[0], f32x2(s.x, s.y));
+      y[1] = mul_f32x2(y[1], f32x2(s.z, s.w));
     }
-    if (g.bias != nullptr) {
-      const uint4 b = *reinterpret_cast<const uint4*>(bias + j);
+    if (has_bias) {
+      const uint2 b = *reinterpret_cast<const uint2*>(bias + j);
       const OutT* e = reinterpret_cast<const OutT*>(&b);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = __fmaf_rn(sa, y[i], out_to_f32<OutT>(e[i]));
+      for (int i = 0; i < 2; ++i)
+        y[i] = fma_f32x2(sa2, y[i],
+                         f32x2(out_to_f32<OutT>(e[2 * i]), out_to_f32<OutT>(e[2 * i + 1])));
     } else if constexpr (FORMAT == TM_FP4_NV) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(sa, y[i]);
+      for (int i = 0; i < 2; ++i) y[i] = mul_f32x2(sa2, y[i]);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r[j + i] = __float_as_uint(y[i]);
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (EPI == TM_EPI_GELU_TANH) y[i] = gelu_f32x2(y[i]);
+      float lo, hi;
+      f32x2_split(y[i], lo, hi);
+      r[j + 2 * i] = __float_as_uint(lo);
+      r[j + 2 * i + 1] = __float_as_uint(hi);
+    }
   }
 }
 
-// Store 32 columns of this lane's row, full 32-byte sectors where the output
+// Store 16 columns of this lane's row, as one 32-byte sector where the output
 // allows it (`wide`: rows start on 32-byte boundaries).  Straight from
-// registers: staged TMA stores wait in the queue of the operand loads, and the
-// epilogue with them (8192 x 12288 x 3072 nvfp4: WIDE_FIGURE).
+// registers: staged TMA stores would wait in the queue of the operand loads.
+// Two 16-byte stores in place of the one cost 8192 x 12288 x 3072 nvfp4
+// 197 against 150 us.
 template <typename OutT>
-__device__ __forceinline__ void pair_store32(OutT* row, const float (&y)[32], int col, int cols,
+__device__ __forceinline__ void pair_store16(OutT* row, const uint32_t* y, int col, int cols,
                                              bool wide) {
+  uint32_t w[8];
 #pragma unroll
-  for (int j = 0; j < 32; j += 16) {
-    uint32_t w[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = pack2<OutT>(y[j + 2 * i], y[j + 2 * i + 1]);
-    OutT* dst = row + col + j;
-    if (wide && col + j + 16 <= cols) {
-      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(w[0]),
-                   "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                   : "memory");
-    } else {  // columns come in multiples of 8
-      if (col + j + 8 <= cols)
-        *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-      if (col + j + 16 <= cols)
-        *reinterpret_cast<uint4*>(dst + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-    }
+  for (int i = 0; i < 8; ++i)
+    w[i] = pack2<OutT>(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]));
+  OutT* dst = row + col;
+  if (wide && col + 16 <= cols) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(w[0]),
+                 "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {  // columns come in multiples of 8
+    if (col + 8 <= cols) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (col + 16 <= cols) *reinterpret_cast<uint4*>(dst + 8) = make_uint4(w[4], w[5], w[6], w[7]);
   }
 }
 
-template <int FORMAT, typename OutT>
+// EPI: 0, TM_EPI_GELU_TANH or TM_EPI_SWIGLU.
+template <int FORMAT, int EPI, typename OutT>
 __global__ void __launch_bounds__(kPairThreads, 1)
     gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tm_a,
                          const __grid_constant__ CUtensorMap tm_b,
@@ -708,6 +725,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       if (!mbar_wait(bar.acc_full, i & 1, bar.abort_flag, g.status)) break;
       tc_fence_after();
       const int64_t row = static_cast<int64_t>(mb) * kPairRows + row_in_tile + lane;
+      const bool in_rows = row < g.M;
+      const uint64_t sa2 = f32x2(sa, sa);
       OutT* out_row = static_cast<OutT*>(g.out) + row * g.ldo;
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
       // the warp's 128 columns, then the accumulator belongs to the next tile
@@ -719,25 +738,20 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(free_leader);
       const int col0 = nb * kPairRows + 128 * h;
-      float y[32];
-      if (g.epilogue & TM_EPI_SWIGLU) {
 #pragma unroll
-        for (int k = 0; k < 4; k += 2) {
-          pair_scale32<FORMAT, OutT>(g, r[k], sa, sb_s + 32 * k, bias_s + 32 * k);
-          pair_scale32<FORMAT, OutT>(g, r[k + 1], sa, sb_s + 32 * k + 32, bias_s + 32 * k + 32);
+      for (int k = 0; k < 4; ++k) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            y[j] = swiglu(__uint_as_float(r[k + (j >> 4)][j & 15]),
-                          __uint_as_float(r[k + (j >> 4)][16 + (j & 15)]));
-          if (row < g.M) pair_store32<OutT>(out_row, y, (col0 + 32 * k) / 2, g.N / 2, g.wide);
+        for (int j = 0; j < 32; j += 16) {
+          pair_finish16<FORMAT, EPI, OutT>(r[k] + j, sa2, g.bias != nullptr, sb_s + 32 * k + j,
+                                           bias_s + 32 * k + j);
+          if (EPI != TM_EPI_SWIGLU && in_rows)
+            pair_store16<OutT>(out_row, r[k] + j, col0 + 32 * k + j, g.N, g.wide);
         }
-      } else {
+        if constexpr (EPI == TM_EPI_SWIGLU) {  // 16 gate columns, then the 16 up columns
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          pair_scale32<FORMAT, OutT>(g, r[k], sa, sb_s + 32 * k, bias_s + 32 * k);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) y[j] = activate(__uint_as_float(r[k][j]), g.epilogue);
-          if (row < g.M) pair_store32<OutT>(out_row, y, col0 + 32 * k, g.N, g.wide);
+          for (int j = 0; j < 16; ++j)
+            r[k][j] = __float_as_uint(swiglu(__uint_as_float(r[k][j]), __uint_as_float(r[k][16 + j])));
+          if (in_rows) pair_store16<OutT>(out_row, r[k], (col0 + 32 * k) / 2, g.N / 2, g.wide);
         }
       }
     }
@@ -816,13 +830,13 @@ int launch_small(const Fp4Operand& x, const Fp4Operand& w, Fp4Args args, int spl
   return check_launch();
 }
 
-// Resident pairs of the pair kernel on a device (cached; both formats and
-// output types need the same resources per CTA but for a few KiB of shared memory).
+// Resident pairs of the pair kernel on a device (cached; its instances differ by
+// a few KiB of shared memory only, one CTA an SM each).
 int max_fp4_pairs(int device, int sms) {
   static int cache[64] = {};
   if (device < 0 || device >= 64) return 0;
   if (cache[device] == 0) {
-    auto kernel = gemm_fp4_pair_kernel<TM_FP4_NV, __nv_bfloat16>;
+    auto kernel = gemm_fp4_pair_kernel<TM_FP4_NV, 0, __nv_bfloat16>;
     constexpr int smem = PairLayout<TM_FP4_NV>::kTotal;
     int clusters = 0;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) ==
@@ -846,7 +860,7 @@ int max_fp4_pairs(int device, int sms) {
   return cache[device] > 0 ? cache[device] : 0;
 }
 
-template <int FORMAT, typename OutT>
+template <int FORMAT, int EPI, typename OutT>
 int launch_pair_fp4(const Fp4Operand& x, const Fp4Operand& w, Fp4Args args, int max_pairs,
                     cudaStream_t stream) {
   using L = PairLayout<FORMAT>;
@@ -861,7 +875,7 @@ int launch_pair_fp4(const Fp4Operand& x, const Fp4Operand& w, Fp4Args args, int 
   if (!encode_codes(&ta, x, args.K, 128) || !encode_codes(&tb, w, args.K, 128) ||
       !encode_scales<FORMAT>(&tas, x, args.K, 1) || !encode_scales<FORMAT>(&tbs, w, args.K, 2))
     return TM_ERR_CUDA;
-  auto kernel = gemm_fp4_pair_kernel<FORMAT, OutT>;
+  auto kernel = gemm_fp4_pair_kernel<FORMAT, EPI, OutT>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal) !=
       cudaSuccess)
     return TM_ERR_CUDA;
@@ -907,7 +921,12 @@ int dispatch_fp4(const Fp4Operand& x, const Fp4Operand& w, const Fp4Args& args, 
     case 32: return launch_small<32, FORMAT, OutT>(x, w, args, c.splits, stream);
     case 64: return launch_small<64, FORMAT, OutT>(x, w, args, c.splits, stream);
     case 128: return launch_small<128, FORMAT, OutT>(x, w, args, c.splits, stream);
-    case kPairTile: return launch_pair_fp4<FORMAT, OutT>(x, w, args, max_pairs, stream);
+    case kPairTile:
+      if (args.epilogue & TM_EPI_GELU_TANH)
+        return launch_pair_fp4<FORMAT, TM_EPI_GELU_TANH, OutT>(x, w, args, max_pairs, stream);
+      if (args.epilogue & TM_EPI_SWIGLU)
+        return launch_pair_fp4<FORMAT, TM_EPI_SWIGLU, OutT>(x, w, args, max_pairs, stream);
+      return launch_pair_fp4<FORMAT, 0, OutT>(x, w, args, max_pairs, stream);
     default: return TM_ERR_UNSUPPORTED;
   }
 }
