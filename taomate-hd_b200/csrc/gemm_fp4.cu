@@ -76,11 +76,6 @@ struct ScaleGeom {
   static constexpr bool kE8m0 = FORMAT == TM_FP4_MX;
 };
 
-// The value of one output before rounding (SwiGLU pairs are combined by the caller).
-__device__ __forceinline__ float activate(float y, uint32_t epilogue) {
-  return (epilogue & TM_EPI_GELU_TANH) ? gelu_tanh(y) : y;
-}
-
 __device__ __forceinline__ float swiglu(float g, float u) {
   return __fmul_rn(__fmul_rn(g, sigmoid_f32(g)), u);
 }
@@ -107,10 +102,16 @@ struct SmallLayout {
   static constexpr int total(int stages, int splits) {
     return 1024 + stages * kStageBytes + kBarBytes + (splits > 1 ? kReduceBytes : 0);
   }
-  // TMEM columns: the accumulator, then two buffers of scale tiles (4 columns each)
-  static constexpr uint32_t kScaleCol = TOK;
-  static constexpr uint32_t kScaleBuf = 2 * 4 * S::kTiles;
-  static constexpr uint32_t kTmemCols = TOK + 2 * kScaleBuf <= 128 ? 128 : 256;
+  // TMEM columns: the accumulator, then each stage's scale tiles (4 columns for
+  // the weight rows and 4 for the tokens), written again after the stage's MMAs
+  static constexpr int kTileCols = 8;
+  static constexpr int kStageCols = kTileCols * S::kTiles;
+  __host__ __device__ static constexpr int tmem_cols(int stages) {
+    int cols = 64;
+    while (cols < TOK + stages * kStageCols) cols *= 2;
+    return cols;
+  }
+  static_assert(TOK + kMaxStages * kStageCols <= 512, "TMEM columns");
 };
 
 struct SmallBars {
@@ -135,18 +136,85 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
-// Store the outputs of token `m` held one weight row per lane: `n` is this
-// lane's output row, y its value before the activation.
+// What a lane of an epilogue warp keeps: its weight row's constants.
+struct RowConsts {
+  int n;
+  float sb, bias;
+};
+
 template <typename OutT>
-__device__ __forceinline__ void store_token(const Fp4Args& g, int64_t m, int n, float y) {
-  OutT* row = static_cast<OutT*>(g.out) + m * g.ldo;
-  if (g.epilogue & TM_EPI_SWIGLU) {
+__device__ __forceinline__ RowConsts row_consts(const Fp4Args& g, int n) {
+  RowConsts c{n, 1.f, 0.f};
+  if (n < g.N) {
+    if (g.sb != nullptr) c.sb = __ldg(g.sb + (g.sb_per_col ? n : 0));
+    if (g.bias != nullptr) c.bias = out_to_f32<OutT>(static_cast<const OutT*>(g.bias)[n]);
+  }
+  return c;
+}
+
+// Finish and store the sums of tokens m and m + 1, a weight row per lane (the
+// lanes of a warp are 32 consecutive output columns).  Neighbouring lanes
+// exchange a value, so that each stores two columns of one token.  `tokens`: 2,
+// or 1 when there is no second token.  Called by the whole warp.
+template <int EPI, typename OutT>
+__device__ __forceinline__ void store_tokens(const Fp4Args& g, const RowConsts& c, int64_t m,
+                                             int tokens, float acc0, float acc1) {
+  const int lane = threadIdx.x & 31;
+  const int64_t m1 = tokens > 1 ? m + 1 : m;
+  const float sa0 = g.sa == nullptr ? 1.f : __ldg(g.sa + (g.sa_per_row ? m : 0));
+  const float sa1 = g.sa == nullptr ? 1.f : __ldg(g.sa + (g.sa_per_row ? m1 : 0));
+  float y0 = __fmaf_rn(sa0, __fmul_rn(c.sb, acc0), c.bias);
+  float y1 = __fmaf_rn(sa1, __fmul_rn(c.sb, acc1), c.bias);
+  int col = c.n;
+  bool in = c.n < g.N;
+  if constexpr (EPI == TM_EPI_GELU_TANH) {
+    y0 = gelu_tanh(y0);
+    y1 = gelu_tanh(y1);
+  } else if constexpr (EPI == TM_EPI_SWIGLU) {
     // weight rows come as 16 gate rows, then the 16 matching up rows
-    const float u = __shfl_down_sync(0xffffffffu, y, 16);
-    if ((threadIdx.x & 16) == 0 && n < g.N)
-      row[(n >> 5) * 16 + (n & 15)] = from_f32<OutT>(swiglu(y, u));
-  } else {
-    if (n < g.N) row[n] = from_f32<OutT>(activate(y, g.epilogue));
+    const float u0 = __shfl_down_sync(0xffffffffu, y0, 16);
+    const float u1 = __shfl_down_sync(0xffffffffu, y1, 16);
+    y0 = swiglu(y0, u0);
+    y1 = swiglu(y1, u1);
+    col = (c.n >> 5) * 16 + (c.n & 15);
+    in = in && lane < 16;
+  }
+  const bool odd = lane & 1;  // odd lanes take the second token
+  const float got = __shfl_xor_sync(0xffffffffu, odd ? y0 : y1, 1);
+  if (in && (!odd || tokens > 1)) {
+    OutT* dst = static_cast<OutT*>(g.out) + (odd ? m1 : m) * g.ldo + (col & ~1);
+    *reinterpret_cast<uint32_t*>(dst) = odd ? pack2<OutT>(got, y1) : pack2<OutT>(y0, got);
+  }
+}
+
+template <int EPI, typename OutT>
+__device__ __forceinline__ void store_tile(const Fp4Args& g, const RowConsts& c, uint32_t t_row,
+                                           int64_t m0, int tokens) {
+#pragma unroll 1
+  for (int t = 0; t < tokens; t += 32) {
+    uint32_t r[32];
+    tmem_ld_32x32b_x32(t_row + t, r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 32; j += 2)
+      if (t + j < tokens)  // the same for the whole warp
+        store_tokens<EPI, OutT>(g, c, m0 + t + j, tokens - t - j, __uint_as_float(r[j]),
+                                __uint_as_float(r[j + 1]));
+  }
+}
+
+// The sums of this CTA's tokens, [slice][token][weight row], added in slice order.
+template <int EPI, typename OutT>
+__device__ __forceinline__ void store_reduced(const Fp4Args& g, const RowConsts& c,
+                                              const float* sums, int splits, int per, int64_t m0,
+                                              int tokens) {
+  for (int t = 0; t < tokens; t += 2) {
+    float a0 = 0.f, a1 = 0.f;
+    for (int s = 0; s < splits; ++s) {
+      a0 += sums[(s * per + t) * kTileRows];
+      if (t + 1 < tokens) a1 += sums[(s * per + t + 1) * kTileRows];
+    }
+    store_tokens<EPI, OutT>(g, c, m0 + t, tokens - t, a0, a1);
   }
 }
 
@@ -173,6 +241,7 @@ __global__ void __launch_bounds__(kSmallThreads)
   // even slices, none empty (splits <= kblocks)
   const int kb0 = static_cast<int>(static_cast<int64_t>(slice) * g.kblocks / splits);
   const int kb1 = static_cast<int>(static_cast<int64_t>(slice + 1) * g.kblocks / splits);
+  const uint32_t tmem_cols = L::tmem_cols(g.stages);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < g.stages; ++s) {
@@ -186,9 +255,17 @@ __global__ void __launch_bounds__(kSmallThreads)
     tma_prefetch_desc(&tm_x);
     tma_prefetch_desc(&tm_ws);
     tma_prefetch_desc(&tm_xs);
+    // With one token tile the weight is read once: ask for this slice of it
+    // while the previous kernel on the stream still runs (an L2 prefetch has
+    // no effect on what is read later, whoever writes the weight).
+    if (g.num_m == 1)
+      for (int kb = kb0; kb < kb1; ++kb) {
+        tma_prefetch_l2_2d(&tm_w, kb * kRowBytes, nb * kTileRows);
+        tma_prefetch_l2_2d(&tm_ws, kb * (S::kBytes / 8), nb);
+      }
   }
   if (warp == 1) {
-    tmem_alloc(bar.tmem_slot, L::kTmemCols);
+    tmem_alloc(bar.tmem_slot, tmem_cols);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -202,17 +279,17 @@ __global__ void __launch_bounds__(kSmallThreads)
   griddep_launch_dependents();
 
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      uint32_t issued_mask = 0, issued_parity = 0;
-      bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&bar.empty[stage], phase ^ 1u, bar.abort_flag, g.status)) {
-          ok = false;
-          break;
-        }
-        issued_mask &= ~(1u << stage);
+    int stage = 0;
+    uint32_t phase = 0;
+    uint32_t issued_mask = 0, issued_parity = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait_warp(&bar.empty[stage], phase ^ 1u, bar.abort_flag, g.status)) {
+        ok = false;
+        break;
+      }
+      issued_mask &= ~(1u << stage);
+      if (elect_one()) {
         uint8_t* s = smem + stage * L::kStageBytes;
         mbar_arrive_expect_tx(&bar.full[stage], L::kStageBytes);
         tma_load_2d(&tm_w, &bar.full[stage], s, kb * kRowBytes, nb * kTileRows);
@@ -220,119 +297,121 @@ __global__ void __launch_bounds__(kSmallThreads)
         tma_load_2d(&tm_x, &bar.full[stage], s + L::kWBytes, kb * kRowBytes, mb * TOK);
         tma_load_2d(&tm_xs, &bar.full[stage], s + L::kWBytes + L::kXBytes + S::kBytes,
                     kb * (S::kBytes / 8), mb);  // TOK = 128, or a single token tile
-        issued_mask |= 1u << stage;
-        issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
-        if (++stage == g.stages) {
-          stage = 0;
-          phase ^= 1u;
-        }
       }
-      if (!ok) {
-        for (int s = 0; s < g.stages; ++s)
-          if (issued_mask & (1u << s))
-            mbar_wait_drain(&bar.full[s], (issued_parity >> s) & 1u, g.status);
+      __syncwarp();
+      issued_mask |= 1u << stage;
+      issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
+      if (++stage == g.stages) {
+        stage = 0;
+        phase ^= 1u;
       }
+    }
+    if (!ok && lane == 0) {
+      for (int s = 0; s < g.stages; ++s)
+        if (issued_mask & (1u << s))
+          mbar_wait_drain(&bar.full[s], (issued_parity >> s) & 1u, g.status);
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      int last = -1, before = -1;  // stages of the previous k-block and of the one before it
-      uint32_t last_phase = 0, before_phase = 0;
-      bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        // the scale buffer was last read two k-blocks ago
-        if (before >= 0 &&
-            !mbar_wait(&bar.empty[before], before_phase, bar.abort_flag, g.status)) {
-          ok = false;
-          break;
+    // the whole warp runs the loop, one lane issues (see elect_one)
+    const uint32_t tmem = __reduce_max_sync(0xffffffffu, tmem_base);
+    const uint32_t smem0 = smem_u32(smem);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true, issued_any = false;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait_warp(&bar.full[stage], phase, bar.abort_flag, g.status)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t base = smem0 + stage * L::kStageBytes;
+      const uint64_t w_desc = make_desc_kmajor_sw128(base);
+      const uint64_t x_desc = make_desc_kmajor_sw128(base + L::kWBytes);
+      const uint64_t ws_desc = make_desc_scale_tile(base + L::kWBytes + L::kXBytes);
+      const uint64_t xs_desc = make_desc_scale_tile(base + L::kWBytes + L::kXBytes + S::kBytes);
+      const uint32_t col = tmem + TOK + stage * L::kStageCols;
+      const uint32_t more = kb != kb0 ? 1u : 0u;
+      const int steps = kblock_steps(g.K, kb);
+      // descriptors count 16-byte units
+      const auto copy = [&](int t) {
+        tmem_copy_scale_tile<false>(col + L::kTileCols * t, ws_desc + 32 * t);
+        tmem_copy_scale_tile<false>(col + L::kTileCols * t + 4, xs_desc + 32 * t);
+      };
+      const auto multiply = [&](int k) {
+        const int t = k / S::kStepsPerTile;
+        umma_fp4<false, S::kBlock>(
+            tmem, w_desc + 2 * k, x_desc + 2 * k,
+            make_idesc_fp4(kTileRows, TOK, S::kE8m0, k % S::kStepsPerTile * 2),
+            col + L::kTileCols * t, col + L::kTileCols * t + 4, k == 0 ? more : 1u);
+      };
+      if (steps == kKBlock / kMmaK) {
+        if (elect_one()) {
+#pragma unroll
+          for (int t = 0; t < S::kTiles; ++t) copy(t);
+#pragma unroll
+          for (int k = 0; k < kKBlock / kMmaK; ++k) multiply(k);
+          umma_commit(&bar.empty[stage]);
         }
-        if (!mbar_wait(&bar.full[stage], phase, bar.abort_flag, g.status)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t w_addr = smem_u32(smem + stage * L::kStageBytes);
-        const uint32_t x_addr = w_addr + L::kWBytes;
-        const uint32_t ws_addr = x_addr + L::kXBytes;
-        const uint32_t xs_addr = ws_addr + S::kBytes;
-        const uint32_t ws_col = tmem_base + L::kScaleCol + ((kb - kb0) & 1) * L::kScaleBuf;
-        const uint32_t xs_col = ws_col + 4 * S::kTiles;
-        const int steps = kblock_steps(g.K, kb);
-        for (int t = 0; t * S::kStepsPerTile < steps; ++t) {
-          tmem_copy_scale_tile<false>(ws_col + 4 * t, make_desc_scale_tile(ws_addr + 512 * t));
-          tmem_copy_scale_tile<false>(xs_col + 4 * t, make_desc_scale_tile(xs_addr + 512 * t));
-        }
-        for (int k = 0; k < steps; ++k) {
-          const int t = k / S::kStepsPerTile, id = k % S::kStepsPerTile * 2;
-          umma_fp4<false, S::kBlock>(tmem_base, make_desc_kmajor_sw128(w_addr + k * 32),
-                                     make_desc_kmajor_sw128(x_addr + k * 32),
-                                     make_idesc_fp4(kTileRows, TOK, S::kE8m0, id), ws_col + 4 * t,
-                                     xs_col + 4 * t, (kb > kb0 || k > 0) ? 1u : 0u);
-        }
-        umma_commit(&bar.empty[stage]);
-        before = last;
-        before_phase = last_phase;
-        last = stage;
-        last_phase = phase;
-        if (++stage == g.stages) {
-          stage = 0;
-          phase ^= 1u;
+      } else {  // the last k-block of a K that is not a multiple of 256
+        if (elect_one()) {
+          for (int t = 0; t * S::kStepsPerTile < steps; ++t) copy(t);
+          for (int k = 0; k < steps; ++k) multiply(k);
+          umma_commit(&bar.empty[stage]);
         }
       }
-      if (ok)
-        umma_commit(bar.acc);
-      else if (last >= 0)
-        mbar_wait_drain(&bar.empty[last], last_phase, g.status);
+      __syncwarp();
+      issued_any = true;
+      if (++stage == g.stages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    if (ok) {
+      if (elect_one()) umma_commit(bar.acc);
+    } else if (issued_any) {  // the last commit: the tensor pipe has drained
+      const int last = stage == 0 ? g.stages - 1 : stage - 1;
+      mbar_wait_drain(&bar.empty[last], stage == 0 ? (phase ^ 1u) : phase, g.status);
     }
     __syncwarp();
   } else {
     const int q = warp & 3;
-    const int n = nb * kTileRows + q * 32 + lane;  // this lane's weight row
-    const float sb = n < g.N ? (g.sb == nullptr ? 1.f : __ldg(g.sb + (g.sb_per_col ? n : 0))) : 0.f;
-    const float bias = (g.bias != nullptr && n < g.N)
-                           ? out_to_f32<OutT>(static_cast<const OutT*>(g.bias)[n])
-                           : 0.f;
     const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
-    const int tokens = min(TOK, g.M - mb * TOK);
-    const bool ok = mbar_wait(bar.acc, 0, bar.abort_flag, g.status);
+    const int64_t m0 = static_cast<int64_t>(mb) * TOK;
+    const int tokens = static_cast<int>(min(static_cast<int64_t>(TOK), g.M - m0));
+    const RowConsts c = row_consts<OutT>(g, nb * kTileRows + q * 32 + lane);
+    const bool ok = mbar_wait_warp(bar.acc, 0, bar.abort_flag, g.status);
     tc_fence_after();
-    const auto token_scale = [&](int64_t m) {
-      return g.sa == nullptr ? 1.f : __ldg(g.sa + (g.sa_per_row ? m : 0));
-    };
     if (splits == 1) {
       if (ok) {
-#pragma unroll 1
-        for (int c = 0; c < tokens; c += 32) {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(t_row + c, r);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            if (c + j < tokens) {  // the same for the whole warp
-              const int64_t m = static_cast<int64_t>(mb) * TOK + c + j;
-              store_token<OutT>(g, m, n,
-                                __fmaf_rn(token_scale(m), __fmul_rn(sb, __uint_as_float(r[j])), bias));
-            }
-          }
-        }
+        if (g.epilogue & TM_EPI_GELU_TANH)
+          store_tile<TM_EPI_GELU_TANH, OutT>(g, c, t_row, m0, tokens);
+        else if (g.epilogue & TM_EPI_SWIGLU)
+          store_tile<TM_EPI_SWIGLU, OutT>(g, c, t_row, m0, tokens);
+        else
+          store_tile<0, OutT>(g, c, t_row, m0, tokens);
       }
     } else {
       // Slice j of the cluster finishes tokens [j, j + 1) * per: send it this
-      // slice's sums of those tokens, [slice][token][weight row].
-      const int per = TOK / splits;
-      const uint32_t mine = smem_u32(reduce);
+      // slice's sums of those tokens.
+      const int per = (tokens + splits - 1) / splits;
+      const uint32_t mine = smem_u32(reduce) + (slice * per * kTileRows + q * 32 + lane) * 4;
 #pragma unroll 1
-      for (int c = 0; c < TOK; c += 32) {
+      for (int t = 0; t < tokens; t += 32) {
         uint32_t r[32];
-        tmem_ld_32x32b_x32(t_row + c, r);
+        tmem_ld_32x32b_x32(t_row + t, r);
         tmem_ld_wait();
+        int to = t / per, at = t - to * per;
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
-          const int to = (c + j) / per, at = (c + j) % per;
-          const uint32_t local = mine + ((slice * per + at) * kTileRows + q * 32 + lane) * 4;
-          st_cluster_f32(map_to_cta(local, to), ok ? __uint_as_float(r[j]) : __int_as_float(0x7fffffff));
+          if (t + j < tokens) {
+            st_cluster_f32(map_to_cta(mine + at * kTileRows * 4, to),
+                           ok ? __uint_as_float(r[j]) : __int_as_float(0x7fffffff));
+            if (++at == per) {
+              at = 0;
+              ++to;
+            }
+          }
         }
       }
     }
@@ -342,29 +421,27 @@ __global__ void __launch_bounds__(kSmallThreads)
   if (splits > 1) {
     cluster_sync();  // every slice's sums have arrived
     if (warp >= 2) {
-      const int q = warp & 3;
-      const int row = q * 32 + lane;
-      const int n = nb * kTileRows + row;
-      const float sb = n < g.N ? (g.sb == nullptr ? 1.f : __ldg(g.sb + (g.sb_per_col ? n : 0))) : 0.f;
-      const float bias = (g.bias != nullptr && n < g.N)
-                             ? out_to_f32<OutT>(static_cast<const OutT*>(g.bias)[n])
-                             : 0.f;
-      const int per = TOK / splits;
-      for (int at = 0; at < per; ++at) {
-        const int64_t m = static_cast<int64_t>(mb) * TOK + slice * per + at;
-        if (m >= g.M) break;
-        float acc = 0.f;
-        for (int s = 0; s < splits; ++s) acc += reduce[(s * per + at) * kTileRows + row];
-        const float sa = g.sa == nullptr ? 1.f : __ldg(g.sa + (g.sa_per_row ? m : 0));
-        store_token<OutT>(g, m, n, __fmaf_rn(sa, __fmul_rn(sb, acc), bias));
-      }
+      const int row = (warp & 3) * 32 + lane;
+      const RowConsts c = row_consts<OutT>(g, nb * kTileRows + row);
+      const int64_t m0 = static_cast<int64_t>(mb) * TOK;
+      const int tokens = static_cast<int>(min(static_cast<int64_t>(TOK), g.M - m0));
+      const int per = (tokens + splits - 1) / splits;
+      const int mine = min(per, tokens - slice * per);  // <= 0: other slices finish them all
+      const float* sums = reduce + row;
+      const int64_t m = m0 + slice * per;
+      if (g.epilogue & TM_EPI_GELU_TANH)
+        store_reduced<TM_EPI_GELU_TANH, OutT>(g, c, sums, splits, per, m, mine);
+      else if (g.epilogue & TM_EPI_SWIGLU)
+        store_reduced<TM_EPI_SWIGLU, OutT>(g, c, sums, splits, per, m, mine);
+      else
+        store_reduced<0, OutT>(g, c, sums, splits, per, m, mine);
     }
   } else {
     __syncthreads();
   }
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, L::kTmemCols);
+    tmem_dealloc(tmem_base, tmem_cols);
   }
 }
 
@@ -791,7 +868,7 @@ bool encode_scales(CUtensorMap* map, const Fp4Operand& op, int64_t k, int row_ti
 constexpr int kSmemBudget = 227 * 1024;
 
 template <int TOK, int FORMAT, typename OutT>
-int launch_small(const Fp4Operand& x, const Fp4Operand& w, Fp4Args args, int splits,
+int launch_small(const Fp4Operand& x, const Fp4Operand& w, Fp4Args args, int splits, int sms,
                  cudaStream_t stream) {
   using L = SmallLayout<TOK, FORMAT>;
   args.num_m = (args.M + TOK - 1) / TOK;
@@ -800,9 +877,13 @@ int launch_small(const Fp4Operand& x, const Fp4Operand& w, Fp4Args args, int spl
   const int longest = (args.kblocks + splits - 1) / splits;
   const int64_t ctas = static_cast<int64_t>(args.num_m) * args.num_n * splits;
   if (ctas > 0x7fffffffLL) return TM_ERR_TOO_LARGE;
-  // two CTAs an SM where that leaves each at least three stages
+  // two CTAs an SM (half the shared memory and TMEM each) once the grid has
+  // more CTAs than SMs, else deeper rings
+  const int budget = ctas > sms ? kSmemBudget / 2 - 1024 : kSmemBudget;
+  const int tmem_budget = ctas > sms ? 256 : 512;
   int stages = kMaxStages;
-  while (stages > 3 && L::total(stages, splits) > kSmemBudget / 2 - 1024) --stages;
+  while (stages > 2 && (L::total(stages, splits) > budget || L::tmem_cols(stages) > tmem_budget))
+    --stages;
   if (stages > longest) stages = longest < 2 ? 2 : longest;
   args.stages = stages;
   CUtensorMap tw, tx, tws, txs;
@@ -916,11 +997,11 @@ Fp4Choice pick_fp4(int64_t m, int64_t n, int kblocks, int sms, int max_pairs) {
 
 template <int FORMAT, typename OutT>
 int dispatch_fp4(const Fp4Operand& x, const Fp4Operand& w, const Fp4Args& args, Fp4Choice c,
-                 int max_pairs, cudaStream_t stream) {
+                 int sms, int max_pairs, cudaStream_t stream) {
   switch (c.tile) {
-    case 32: return launch_small<32, FORMAT, OutT>(x, w, args, c.splits, stream);
-    case 64: return launch_small<64, FORMAT, OutT>(x, w, args, c.splits, stream);
-    case 128: return launch_small<128, FORMAT, OutT>(x, w, args, c.splits, stream);
+    case 32: return launch_small<32, FORMAT, OutT>(x, w, args, c.splits, sms, stream);
+    case 64: return launch_small<64, FORMAT, OutT>(x, w, args, c.splits, sms, stream);
+    case 128: return launch_small<128, FORMAT, OutT>(x, w, args, c.splits, sms, stream);
     case kPairTile:
       if (args.epilogue & TM_EPI_GELU_TANH)
         return launch_pair_fp4<FORMAT, TM_EPI_GELU_TANH, OutT>(x, w, args, max_pairs, stream);
@@ -983,10 +1064,10 @@ int scaled_mm_fp4_impl(void* out, int out_dtype, const uint8_t* a, const uint8_t
   const cudaStream_t st = as_stream(stream);
   const bool bf16 = out_dtype == TM_DTYPE_BF16;
   if (format == TM_FP4_NV)
-    return bf16 ? dispatch_fp4<TM_FP4_NV, __nv_bfloat16>(x, w, args, c, max_pairs, st)
-                : dispatch_fp4<TM_FP4_NV, __half>(x, w, args, c, max_pairs, st);
-  return bf16 ? dispatch_fp4<TM_FP4_MX, __nv_bfloat16>(x, w, args, c, max_pairs, st)
-              : dispatch_fp4<TM_FP4_MX, __half>(x, w, args, c, max_pairs, st);
+    return bf16 ? dispatch_fp4<TM_FP4_NV, __nv_bfloat16>(x, w, args, c, sms, max_pairs, st)
+                : dispatch_fp4<TM_FP4_NV, __half>(x, w, args, c, sms, max_pairs, st);
+  return bf16 ? dispatch_fp4<TM_FP4_MX, __nv_bfloat16>(x, w, args, c, sms, max_pairs, st)
+              : dispatch_fp4<TM_FP4_MX, __half>(x, w, args, c, sms, max_pairs, st);
 }
 
 }  // namespace
