@@ -4,6 +4,7 @@
 // links only the CUDA runtime).
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -35,6 +36,19 @@ inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s
 
 inline int check_launch() {
   return cudaGetLastError() == cudaSuccess ? TM_OK : TM_ERR_CUDA;
+}
+
+// Allow `kernel` dynamic shared memory of up to `bytes`, once per device
+// (`done`: a static array of the call site).  Losing a race repeats the call.
+template <typename Kernel>
+bool allow_smem(Kernel kernel, int bytes, int device, std::atomic<bool> (&done)[64]) {
+  const bool known = device >= 0 && device < 64;
+  if (known && done[device].load(std::memory_order_acquire)) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+      cudaSuccess)
+    return false;
+  if (known) done[device].store(true, std::memory_order_release);
+  return true;
 }
 
 // Launch with programmatic dependent launch allowed (the kernel calls

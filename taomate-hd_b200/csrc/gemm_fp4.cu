@@ -843,6 +843,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 }
 
 // ====================================================================== host
+struct Fp4Device {
+  int id, sms, max_pairs;
+};
+
 struct Fp4Operand {
   const uint8_t* codes;
   int64_t ld;  // bytes
@@ -868,8 +872,8 @@ bool encode_scales(CUtensorMap* map, const Fp4Operand& op, int64_t k, int row_ti
 constexpr int kSmemBudget = 227 * 1024;
 
 template <int TOK, int FORMAT, typename OutT>
-int launch_small(const Fp4Operand& x, const Fp4Operand& w, Fp4Args args, int splits, int sms,
-                 cudaStream_t stream) {
+int launch_small(const Fp4Operand& x, const Fp4Operand& w, Fp4Args args, int splits,
+                 const Fp4Device& dev, cudaStream_t stream) {
   using L = SmallLayout<TOK, FORMAT>;
   args.num_m = (args.M + TOK - 1) / TOK;
   args.num_n = (args.N + kTileRows - 1) / kTileRows;
@@ -879,8 +883,8 @@ int launch_small(const Fp4Operand& x, const Fp4Operand& w, Fp4Args args, int spl
   if (ctas > 0x7fffffffLL) return TM_ERR_TOO_LARGE;
   // two CTAs an SM (half the shared memory and TMEM each) once the grid has
   // more CTAs than SMs, else deeper rings
-  const int budget = ctas > sms ? kSmemBudget / 2 - 1024 : kSmemBudget;
-  const int tmem_budget = ctas > sms ? 256 : 512;
+  const int budget = ctas > dev.sms ? kSmemBudget / 2 - 1024 : kSmemBudget;
+  const int tmem_budget = ctas > dev.sms ? 256 : 512;
   int stages = kMaxStages;
   while (stages > 2 && (L::total(stages, splits) > budget || L::tmem_cols(stages) > tmem_budget))
     --stages;
@@ -892,9 +896,8 @@ int launch_small(const Fp4Operand& x, const Fp4Operand& w, Fp4Args args, int spl
     return TM_ERR_CUDA;
   auto kernel = gemm_fp4_small_kernel<TOK, FORMAT, OutT>;
   const int smem = L::total(stages, splits);
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBudget) !=
-      cudaSuccess)
-    return TM_ERR_CUDA;
+  static std::atomic<bool> allowed[64] = {};
+  if (!allow_smem(kernel, kSmemBudget, dev.id, allowed)) return TM_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(kSmallThreads);
@@ -942,10 +945,10 @@ int max_fp4_pairs(int device, int sms) {
 }
 
 template <int FORMAT, int EPI, typename OutT>
-int launch_pair_fp4(const Fp4Operand& x, const Fp4Operand& w, Fp4Args args, int max_pairs,
+int launch_pair_fp4(const Fp4Operand& x, const Fp4Operand& w, Fp4Args args, const Fp4Device& dev,
                     cudaStream_t stream) {
   using L = PairLayout<FORMAT>;
-  if (max_pairs <= 0) return TM_ERR_UNSUPPORTED;
+  if (dev.max_pairs <= 0) return TM_ERR_UNSUPPORTED;
   args.num_m = (args.M + kPairRows - 1) / kPairRows;
   args.num_n = (args.N + kPairRows - 1) / kPairRows;
   args.group_n = choose_group_n(args.num_n, kPairRows, kPairRows, args.K / 2);
@@ -957,10 +960,9 @@ int launch_pair_fp4(const Fp4Operand& x, const Fp4Operand& w, Fp4Args args, int 
       !encode_scales<FORMAT>(&tas, x, args.K, 1) || !encode_scales<FORMAT>(&tbs, w, args.K, 2))
     return TM_ERR_CUDA;
   auto kernel = gemm_fp4_pair_kernel<FORMAT, EPI, OutT>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal) !=
-      cudaSuccess)
-    return TM_ERR_CUDA;
-  const int pairs = static_cast<int>(tiles < max_pairs ? tiles : max_pairs);
+  static std::atomic<bool> allowed[64] = {};
+  if (!allow_smem(kernel, L::kTotal, dev.id, allowed)) return TM_ERR_CUDA;
+  const int pairs = static_cast<int>(tiles < dev.max_pairs ? tiles : dev.max_pairs);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
   cfg.blockDim = dim3(kPairThreads);
@@ -986,28 +988,27 @@ struct Fp4Choice {
   int splits;
 };
 
-Fp4Choice pick_fp4(int64_t m, int64_t n, int kblocks, int sms, int max_pairs) {
-  if (m > 128 && max_pairs > 0 && ((m + 255) / 256) * ((n + 255) / 256) * 2 >= max_pairs)
-    return Fp4Choice{kPairTile, 1};
+Fp4Choice pick_fp4(int64_t m, int64_t n, int kblocks, const Fp4Device& dev) {
+  if (m > 64 && dev.max_pairs > 0) return Fp4Choice{kPairTile, 1};
   Fp4Choice c{m <= 32 ? 32 : m <= 64 ? 64 : 128, 1};
   const int64_t tiles = (m + c.tile - 1) / c.tile * ((n + kTileRows - 1) / kTileRows);
-  while (c.splits < 8 && tiles * c.splits * 2 <= 2 * sms && kblocks >= 4 * c.splits) c.splits *= 2;
+  while (c.splits < 8 && tiles * c.splits < dev.sms / 2 && kblocks >= 4 * c.splits) c.splits *= 2;
   return c;
 }
 
 template <int FORMAT, typename OutT>
 int dispatch_fp4(const Fp4Operand& x, const Fp4Operand& w, const Fp4Args& args, Fp4Choice c,
-                 int sms, int max_pairs, cudaStream_t stream) {
+                 const Fp4Device& dev, cudaStream_t stream) {
   switch (c.tile) {
-    case 32: return launch_small<32, FORMAT, OutT>(x, w, args, c.splits, sms, stream);
-    case 64: return launch_small<64, FORMAT, OutT>(x, w, args, c.splits, sms, stream);
-    case 128: return launch_small<128, FORMAT, OutT>(x, w, args, c.splits, sms, stream);
+    case 32: return launch_small<32, FORMAT, OutT>(x, w, args, c.splits, dev, stream);
+    case 64: return launch_small<64, FORMAT, OutT>(x, w, args, c.splits, dev, stream);
+    case 128: return launch_small<128, FORMAT, OutT>(x, w, args, c.splits, dev, stream);
     case kPairTile:
       if (args.epilogue & TM_EPI_GELU_TANH)
-        return launch_pair_fp4<FORMAT, TM_EPI_GELU_TANH, OutT>(x, w, args, max_pairs, stream);
+        return launch_pair_fp4<FORMAT, TM_EPI_GELU_TANH, OutT>(x, w, args, dev, stream);
       if (args.epilogue & TM_EPI_SWIGLU)
-        return launch_pair_fp4<FORMAT, TM_EPI_SWIGLU, OutT>(x, w, args, max_pairs, stream);
-      return launch_pair_fp4<FORMAT, 0, OutT>(x, w, args, max_pairs, stream);
+        return launch_pair_fp4<FORMAT, TM_EPI_SWIGLU, OutT>(x, w, args, dev, stream);
+      return launch_pair_fp4<FORMAT, 0, OutT>(x, w, args, dev, stream);
     default: return TM_ERR_UNSUPPORTED;
   }
 }
@@ -1052,10 +1053,10 @@ int scaled_mm_fp4_impl(void* out, int out_dtype, const uint8_t* a, const uint8_t
   args.kblocks = static_cast<int>((k + kKBlock - 1) / kKBlock);
   args.epilogue = epilogue;
   args.status = device_status_ptr(device);
-  const int max_pairs = max_fp4_pairs(device, sms);
+  const Fp4Device dev{device, sms, max_fp4_pairs(device, sms)};
   Fp4Choice c{tile, splits};
   if (tile == 0) {
-    c = pick_fp4(m, n, args.kblocks, sms, max_pairs);
+    c = pick_fp4(m, n, args.kblocks, dev);
   } else {
     if (splits != 1 && splits != 2 && splits != 4 && splits != 8) return TM_ERR_UNSUPPORTED;
     if ((tile < 128 && m > tile) || (tile == kPairTile && splits != 1)) return TM_ERR_UNSUPPORTED;
@@ -1064,10 +1065,10 @@ int scaled_mm_fp4_impl(void* out, int out_dtype, const uint8_t* a, const uint8_t
   const cudaStream_t st = as_stream(stream);
   const bool bf16 = out_dtype == TM_DTYPE_BF16;
   if (format == TM_FP4_NV)
-    return bf16 ? dispatch_fp4<TM_FP4_NV, __nv_bfloat16>(x, w, args, c, sms, max_pairs, st)
-                : dispatch_fp4<TM_FP4_NV, __half>(x, w, args, c, sms, max_pairs, st);
-  return bf16 ? dispatch_fp4<TM_FP4_MX, __nv_bfloat16>(x, w, args, c, sms, max_pairs, st)
-              : dispatch_fp4<TM_FP4_MX, __half>(x, w, args, c, sms, max_pairs, st);
+    return bf16 ? dispatch_fp4<TM_FP4_NV, __nv_bfloat16>(x, w, args, c, dev, st)
+                : dispatch_fp4<TM_FP4_NV, __half>(x, w, args, c, dev, st);
+  return bf16 ? dispatch_fp4<TM_FP4_MX, __nv_bfloat16>(x, w, args, c, dev, st)
+              : dispatch_fp4<TM_FP4_MX, __half>(x, w, args, c, dev, st);
 }
 
 }  // namespace

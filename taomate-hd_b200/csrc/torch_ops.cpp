@@ -9,6 +9,8 @@
 // cutlass_scaled_mm / scaled_mm_i8_ex (cached per device and stream, from
 // torch's caching allocator) for shapes that use split-K.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/empty_like.h>
 #include <ATen/ops/zeros.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
@@ -726,6 +728,115 @@ void scaled_mm_fp4(at::Tensor& out, const at::Tensor& a, const at::Tensor& b,
   check_status(status, "scaled_mm_fp4");
 }
 
+// ---- the allocating forms, one dispatcher call each (the Python API) ----
+struct Fp4Tensors {
+  at::Tensor q, blocks;
+  std::optional<at::Tensor> scales;
+};
+
+Fp4Tensors empty_fp4(const at::Tensor& like, bool mx, bool row_scales) {
+  TORCH_CHECK(like.dim() >= 1, "input must have at least one dimension");
+  const int64_t cols = like.size(-1);
+  TORCH_CHECK(cols > 0 && cols % 32 == 0,
+              "4-bit rows must be a positive multiple of 32 elements wide, got ", cols);
+  const int64_t rows = like.numel() / cols;
+  Fp4Tensors t;
+  at::DimVector sizes(like.sizes());
+  sizes.back() = cols / 2;
+  t.q = at::empty(sizes, like.options().dtype(at::kByte));
+  const int64_t blocks = cols / (mx ? 32 : 16);
+  t.blocks = at::empty({(rows + 127) / 128 * 128, (blocks + 3) / 4 * 4},
+                       like.options().dtype(mx ? at::kFloat8_e8m0fnu : at::kFloat8_e4m3fn));
+  if (row_scales && !mx) t.scales = at::empty({rows, 1}, like.options().dtype(at::kFloat));
+  return t;
+}
+
+using Fp4Result = std::tuple<at::Tensor, at::Tensor, std::optional<at::Tensor>>;
+
+Fp4Result scaled_fp4_quant_new(const at::Tensor& input, const std::optional<at::Tensor>& scale,
+                               bool mx) {
+  TORCH_CHECK(!mx || !scale.has_value(), "blocks of 32 take no fp32 scale");
+  const c10::cuda::CUDAGuard guard(input.device());
+  Fp4Tensors t = empty_fp4(input, mx, !scale.has_value());
+  const bool rows = input.dim() == 2 && input.stride(1) == 1;
+  scaled_fp4_quant(t.q, t.blocks, t.scales, rows ? input : input.contiguous(), scale);
+  return {t.q, t.blocks, scale.has_value() ? scale : t.scales};
+}
+
+at::Tensor dequantize_fp4_new(const at::Tensor& q, const at::Tensor& block_scales,
+                              const std::optional<at::Tensor>& scales, at::ScalarType dtype) {
+  TORCH_CHECK(q.dim() >= 1, "q must have at least one dimension");
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::DimVector sizes(q.sizes());
+  sizes.back() *= 2;
+  at::Tensor out = at::empty(sizes, q.options().dtype(dtype));
+  dequantize_fp4(out, q.contiguous(), block_scales, scales);
+  return out;
+}
+
+at::Tensor scaled_mm_fp4_new(const at::Tensor& a, const at::Tensor& b,
+                             const at::Tensor& block_scales_a, const at::Tensor& block_scales_b,
+                             const std::optional<at::Tensor>& scales_a,
+                             const std::optional<at::Tensor>& scales_b, at::ScalarType dtype,
+                             const std::optional<at::Tensor>& bias, int64_t epilogue) {
+  TORCH_CHECK(a.dim() >= 1 && a.size(-1) > 0, "a must be [..., K / 2] with K > 0");
+  TORCH_CHECK(b.dim() == 2, "b must be 2-D");
+  const c10::cuda::CUDAGuard guard(a.device());
+  const at::Tensor a2 = a.dim() == 2 ? a : a.reshape({a.numel() / a.size(-1), a.size(-1)});
+  const int64_t cols = (epilogue & TM_EPI_SWIGLU) ? b.size(1) / 2 : b.size(1);
+  at::Tensor out = at::empty({a2.size(0), cols}, a.options().dtype(dtype));
+  scaled_mm_fp4(out, a2, b, block_scales_a, block_scales_b, scales_a, scales_b, bias, epilogue, 0,
+                1);
+  if (a.dim() == 2) return out;
+  at::DimVector sizes(a.sizes());
+  sizes.back() = cols;
+  return out.view(sizes);
+}
+
+using Fp4Hidden =
+    std::tuple<at::Tensor, at::Tensor, std::optional<at::Tensor>, std::optional<at::Tensor>>;
+
+std::optional<at::Tensor> empty_hidden(const at::Tensor& x, bool wanted) {
+  return wanted ? std::optional<at::Tensor>(at::empty_like(x)) : std::nullopt;
+}
+
+Fp4Hidden modulate_fp4_quant_new(const at::Tensor& x, const at::Tensor& shift,
+                                 const at::Tensor& scale, const std::optional<at::Tensor>& index,
+                                 bool mx, bool hidden) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  Fp4Tensors t = empty_fp4(x, mx, true);
+  const std::optional<at::Tensor> h = empty_hidden(x, hidden);
+  modulate_fp4_quant(t.q, t.blocks, t.scales, h, x, shift, scale, index);
+  return {t.q, t.blocks, t.scales, h};
+}
+
+Fp4Hidden rms_norm_modulate_fp4_quant_new(const at::Tensor& x, const at::Tensor& weight, double eps,
+                                          const at::Tensor& shift, const at::Tensor& scale,
+                                          const std::optional<at::Tensor>& index, bool mx,
+                                          bool hidden) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  Fp4Tensors t = empty_fp4(x, mx, true);
+  const std::optional<at::Tensor> h = empty_hidden(x, hidden);
+  rms_norm_modulate_fp4_quant(t.q, t.blocks, t.scales, h, x, weight, eps, shift, scale, index);
+  return {t.q, t.blocks, t.scales, h};
+}
+
+std::tuple<at::Tensor, at::Tensor, std::optional<at::Tensor>, at::Tensor, std::optional<at::Tensor>>
+residual_gate_rms_norm_modulate_fp4_quant_new(const at::Tensor& residual, const at::Tensor& branch,
+                                              const at::Tensor& gate, const at::Tensor& weight,
+                                              double eps, const at::Tensor& shift,
+                                              const at::Tensor& scale,
+                                              const std::optional<at::Tensor>& index, bool mx,
+                                              bool hidden) {
+  const c10::cuda::CUDAGuard guard(residual.device());
+  Fp4Tensors t = empty_fp4(residual, mx, true);
+  const std::optional<at::Tensor> h = empty_hidden(residual, hidden);
+  at::Tensor residual_out = at::empty_like(residual);
+  residual_gate_rms_norm_modulate_fp4_quant(t.q, t.blocks, t.scales, residual_out, h, residual,
+                                            branch, gate, weight, eps, shift, scale, index);
+  return {t.q, t.blocks, t.scales, residual_out, h};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(taomate_w8a8, m) {
@@ -776,6 +887,25 @@ TORCH_LIBRARY(taomate_w8a8, m) {
       "scaled_mm_fp4(Tensor(a!) out, Tensor a, Tensor b, Tensor block_scales_a, "
       "Tensor block_scales_b, Tensor? scales_a, Tensor? scales_b, Tensor? bias, int epilogue, "
       "int tile, int splits) -> ()");
+  m.def(
+      "scaled_fp4_quant_new(Tensor input, Tensor? scale, bool mx) -> (Tensor, Tensor, Tensor?)");
+  m.def(
+      "dequantize_fp4_new(Tensor q, Tensor block_scales, Tensor? scales, ScalarType dtype) -> "
+      "Tensor");
+  m.def(
+      "scaled_mm_fp4_new(Tensor a, Tensor b, Tensor block_scales_a, Tensor block_scales_b, "
+      "Tensor? scales_a, Tensor? scales_b, ScalarType dtype, Tensor? bias, int epilogue) -> "
+      "Tensor");
+  m.def(
+      "modulate_fp4_quant_new(Tensor x, Tensor shift, Tensor scale, Tensor? index, bool mx, "
+      "bool hidden) -> (Tensor, Tensor, Tensor?, Tensor?)");
+  m.def(
+      "rms_norm_modulate_fp4_quant_new(Tensor x, Tensor weight, float eps, Tensor shift, "
+      "Tensor scale, Tensor? index, bool mx, bool hidden) -> (Tensor, Tensor, Tensor?, Tensor?)");
+  m.def(
+      "residual_gate_rms_norm_modulate_fp4_quant_new(Tensor residual, Tensor branch, Tensor gate, "
+      "Tensor weight, float eps, Tensor shift, Tensor scale, Tensor? index, bool mx, bool hidden) "
+      "-> (Tensor, Tensor, Tensor?, Tensor, Tensor?)");
 }
 
 TORCH_LIBRARY_IMPL(taomate_w8a8, CUDA, m) {
@@ -797,4 +927,11 @@ TORCH_LIBRARY_IMPL(taomate_w8a8, CUDA, m) {
   m.impl("rms_norm_modulate_fp4_quant", &rms_norm_modulate_fp4_quant);
   m.impl("residual_gate_rms_norm_modulate_fp4_quant", &residual_gate_rms_norm_modulate_fp4_quant);
   m.impl("scaled_mm_fp4", &scaled_mm_fp4);
+  m.impl("scaled_fp4_quant_new", &scaled_fp4_quant_new);
+  m.impl("dequantize_fp4_new", &dequantize_fp4_new);
+  m.impl("scaled_mm_fp4_new", &scaled_mm_fp4_new);
+  m.impl("modulate_fp4_quant_new", &modulate_fp4_quant_new);
+  m.impl("rms_norm_modulate_fp4_quant_new", &rms_norm_modulate_fp4_quant_new);
+  m.impl("residual_gate_rms_norm_modulate_fp4_quant_new",
+         &residual_gate_rms_norm_modulate_fp4_quant_new);
 }

@@ -183,26 +183,10 @@ def lora_down_proj(x: torch.Tensor, a: torch.Tensor, *,
     return out
 
 
-_FP4_BLOCK_DTYPES = {"nvfp4": (16, torch.float8_e4m3fn), "mxfp4": (32, torch.float8_e8m0fnu)}
-
-
-def _empty_fp4(
-    like: torch.Tensor, block_format: str, row_scales: bool
-) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
-    """Uninitialised ``(codes, block scales, row scales or None)`` for a tensor like ``like``."""
-    if block_format not in _FP4_BLOCK_DTYPES:
-        raise ValueError(f"block_format must be one of {sorted(_FP4_BLOCK_DTYPES)}")
-    block, dtype = _FP4_BLOCK_DTYPES[block_format]
-    cols = like.shape[-1] if like.dim() else 0
-    if cols == 0 or cols % 32:
-        raise ValueError(f"4-bit rows must be a positive multiple of 32 elements wide, got {cols}")
-    rows = like.numel() // cols
-    q = torch.empty((*like.shape[:-1], cols // 2), dtype=torch.uint8, device=like.device)
-    tiles = (-(-rows // 128) * 128, -(-(cols // block) // 4) * 4)
-    block_scales = torch.empty(tiles, dtype=torch.uint8, device=like.device).view(dtype)
-    scales = (torch.empty((rows, 1), dtype=torch.float32, device=like.device)
-              if row_scales and block_format == "nvfp4" else None)
-    return q, block_scales, scales
+def _is_mx(block_format: str) -> bool:
+    if block_format not in ("nvfp4", "mxfp4"):
+        raise ValueError("block_format must be 'nvfp4' or 'mxfp4'")
+    return block_format == "mxfp4"
 
 
 def scaled_fp4_quant(
@@ -232,12 +216,7 @@ def scaled_fp4_quant(
     infinity or a NaN becomes NaN as a whole.
     """
     _require_cuda(input, scale)
-    q, block_scales, scales = _empty_fp4(input, block_format, scale is None)
-    if scale is not None and block_format != "nvfp4":
-        raise ValueError("only nvfp4 takes an fp32 scale")
-    x = input if input.dim() == 2 and input.stride(1) == 1 else input.contiguous()
-    _ops.scaled_fp4_quant(q, block_scales, scales, x, scale)
-    return q, block_scales, scales if scale is None else scale
+    return _ops.scaled_fp4_quant_new.default(input, scale, _is_mx(block_format))
 
 
 def dequantize_fp4(
@@ -249,9 +228,7 @@ def dequantize_fp4(
     """The values of a tensor quantised by :func:`scaled_fp4_quant`, ``[..., K]``
     in ``out_dtype`` (bf16, fp16 or fp32): what a layer would see at 4 bits."""
     _require_cuda(q, block_scales, scales)
-    out = torch.empty((*q.shape[:-1], 2 * q.shape[-1]), dtype=out_dtype, device=q.device)
-    _ops.dequantize_fp4(out, q.contiguous(), block_scales, scales)
-    return out
+    return _ops.dequantize_fp4_new.default(q, block_scales, scales, out_dtype)
 
 
 def scaled_mm_fp4(
@@ -285,18 +262,17 @@ def scaled_mm_fp4(
     _require_cuda(a, b, block_scale_a, block_scale_b, scale_a, scale_b, bias, out)
     if gelu_tanh and swiglu:
         raise ValueError("gelu_tanh and swiglu are exclusive")
-    if a.dim() == 0 or a.shape[-1] == 0:
-        raise ValueError("a must be [..., K / 2] with K > 0")
-    a2 = a if a.dim() == 2 else a.reshape(-1, a.shape[-1])
-    shape = None
+    epi = (EPI_GELU_TANH if gelu_tanh else 0) | (EPI_SWIGLU if swiglu else 0)
+    if out is None and tile == 0:
+        return _ops.scaled_mm_fp4_new.default(a, b, block_scale_a, block_scale_b, scale_a, scale_b,
+                                              out_dtype, bias, epi)
+    a2 = a.reshape(-1, a.shape[-1])
     if out is None:
         cols = b.shape[1] // 2 if swiglu else b.shape[1]
-        shape = (*a.shape[:-1], cols)
         out = torch.empty((a2.shape[0], cols), dtype=out_dtype, device=a.device)
-    epi = (EPI_GELU_TANH if gelu_tanh else 0) | (EPI_SWIGLU if swiglu else 0)
-    _ops.scaled_mm_fp4(out, a2, b, block_scale_a, block_scale_b, scale_a, scale_b, bias, epi, tile,
-                       splits)
-    return out if shape is None else out.view(shape)
+    _ops.scaled_mm_fp4.default(out, a2, b, block_scale_a, block_scale_b, scale_a, scale_b, bias,
+                               epi, tile, splits)
+    return out
 
 
 def quantize_weight_int8(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -464,10 +440,8 @@ def modulate_fp4_quant(
     block_scales, scales or None, hidden or None)``, the hidden state the same
     bits as the int8 producer's, quantised as by :func:`scaled_fp4_quant`."""
     _require_cuda(x, shift, scale, index)
-    q, b, s = _empty_fp4(x, block_format, True)
-    hidden = torch.empty_like(x) if return_hidden else None
-    _ops.modulate_fp4_quant(q, b, s, hidden, x, shift, scale, index)
-    return q, b, s, hidden
+    return _ops.modulate_fp4_quant_new.default(x, shift, scale, index, _is_mx(block_format),
+                                               return_hidden)
 
 
 def rms_norm_modulate_fp4_quant(
@@ -484,10 +458,8 @@ def rms_norm_modulate_fp4_quant(
     """:func:`rms_norm_modulate_int8_quant` with 4-bit output
     (:func:`modulate_fp4_quant`)."""
     _require_cuda(x, weight, shift, scale, index)
-    q, b, s = _empty_fp4(x, block_format, True)
-    hidden = torch.empty_like(x) if return_hidden else None
-    _ops.rms_norm_modulate_fp4_quant(q, b, s, hidden, x, weight, float(eps), shift, scale, index)
-    return q, b, s, hidden
+    return _ops.rms_norm_modulate_fp4_quant_new.default(
+        x, weight, float(eps), shift, scale, index, _is_mx(block_format), return_hidden)
 
 
 def residual_gate_rms_norm_modulate_fp4_quant(
@@ -507,10 +479,6 @@ def residual_gate_rms_norm_modulate_fp4_quant(
     returns ``(codes, block_scales, scales or None, updated residual, hidden
     or None)``."""
     _require_cuda(residual, branch, gate, weight, shift, scale, index)
-    q, b, s = _empty_fp4(residual, block_format, True)
-    residual_out = torch.empty_like(residual)
-    hidden = torch.empty_like(residual) if return_hidden else None
-    _ops.residual_gate_rms_norm_modulate_fp4_quant(
-        q, b, s, residual_out, hidden, residual, branch, gate, weight, float(eps), shift, scale,
-        index)
-    return q, b, s, residual_out, hidden
+    return _ops.residual_gate_rms_norm_modulate_fp4_quant_new.default(
+        residual, branch, gate, weight, float(eps), shift, scale, index, _is_mx(block_format),
+        return_hidden)
