@@ -103,44 +103,6 @@ __device__ __forceinline__ uint32_t nv_scale_byte(float m, float o, float inv6o)
   return d > 0.0f || (d == 0.0f && (lo & 1u)) ? hi : lo;
 }
 
-// Resolve the codes of eight values that lie within 2^-21 of a border: lo and
-// hi are the conversions from just below and just above.
-__device__ __forceinline__ uint32_t resolve8(uint32_t lo, uint32_t hi, const float (&x)[8], float s,
-                                             float o) {
-  uint32_t out = lo;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t a = (lo >> (4 * j)) & 7u, b = (hi >> (4 * j)) & 7u;
-    if (a != b) {
-      const float ts = __fmul_rn(0.5f * (e2m1_value(a) + e2m1_value(b)), s);
-      const float d = __fmaf_rn(-ts, o, fabsf(x[j]));
-      if (d > 0.0f || (d == 0.0f && (a & 1u)))
-        out = (out & ~(7u << (4 * j))) | (b << (4 * j));
-    }
-  }
-  return out;
-}
-
-// Eight codes of x under block scale s and outer scale o; inv = 1 / (o s).
-__device__ __forceinline__ uint32_t nv_codes8(const float (&x)[8], float inv, float s, float o) {
-  const float below = __fmul_rn(inv, kBelow), above = __fmul_rn(inv, kAbove);
-  float a[8], b[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    a[j] = __fmul_rn(x[j], below);
-    b[j] = __fmul_rn(x[j], above);
-  }
-  const uint32_t lo = e2m1x8(a), hi = e2m1x8(b);
-  return lo == hi ? lo : resolve8(lo, hi, x, s, o);
-}
-
-__device__ __forceinline__ uint32_t mx_codes8(const float (&x)[8], float inv) {
-  float a[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) a[j] = __fmul_rn(x[j], inv);  // exact, or far below the first border
-  return e2m1x8(a);
-}
-
 // ---- a thread's 16 elements ----
 template <typename T>
 struct Unit {  // 16-bit types: 16 values in 32 bytes
@@ -151,10 +113,69 @@ struct Unit<float> {
   uint4 raw[4];
 };
 
-// 32 bytes; `wide`: the address is a multiple of 32 (one load), else of 16.
+// Value j (0..7) of a half unit, picked at run time without indexing memory.
+template <typename T>
+__device__ __forceinline__ float unit_value(const Unit<T>& u, int half, int j) {
+  if constexpr (sizeof(T) == 2) {
+    const uint4& r = u.raw[half];
+    const uint32_t w = j < 4 ? (j < 2 ? r.x : r.y) : (j < 6 ? r.z : r.w);
+    const uint16_t e = static_cast<uint16_t>(j & 1 ? w >> 16 : w);
+    return to_f32<T>(*reinterpret_cast<const T*>(&e));
+  } else {
+    const uint4 &a = u.raw[2 * half], &b = u.raw[2 * half + 1];
+    const uint32_t x = j < 4 ? a.x : b.x, y = j < 4 ? a.y : b.y;
+    const uint32_t z = j < 4 ? a.z : b.z, w = j < 4 ? a.w : b.w;
+    return __uint_as_float((j & 2) ? (j & 1 ? w : z) : (j & 1 ? y : x));
+  }
+}
+
+// Decide the codes that differ between lo and hi (the conversions from just
+// below and just above a value): the value lies within 2^-21 of a border.
+template <typename T>
+__device__ __forceinline__ uint32_t resolve8(uint32_t lo, uint32_t hi, const Unit<T>& u, int half,
+                                             float s, float o) {
+  uint32_t left = lo ^ hi;
+  do {
+    const int j = (__ffs(left) - 1) >> 2;
+    const uint32_t a = (lo >> (4 * j)) & 7u, b = (hi >> (4 * j)) & 7u;
+    const float ts = __fmul_rn(0.5f * (e2m1_value(a) + e2m1_value(b)), s);
+    const float d = __fmaf_rn(-ts, o, fabsf(unit_value(u, half, j)));
+    if (d > 0.0f || (d == 0.0f && (a & 1u))) lo = (lo & ~(7u << (4 * j))) | (b << (4 * j));
+    left &= ~(15u << (4 * j));
+  } while (left != 0u);
+  return lo;
+}
+
+// Eight codes of a half unit under block scale s and outer scale o; inv = 1 / (o s).
+template <typename T>
+__device__ __forceinline__ uint32_t nv_codes8(const Unit<T>& u, int half, const float (&x)[8],
+                                              float inv, float s, float o) {
+  const uint64_t below = f32x2(__fmul_rn(inv, kBelow), __fmul_rn(inv, kBelow));
+  const uint64_t above = f32x2(__fmul_rn(inv, kAbove), __fmul_rn(inv, kAbove));
+  float a[8], b[8];
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    const uint64_t v = f32x2(x[j], x[j + 1]);
+    f32x2_split(mul_f32x2(v, below), a[j], a[j + 1]);
+    f32x2_split(mul_f32x2(v, above), b[j], b[j + 1]);
+  }
+  const uint32_t lo = e2m1x8(a), hi = e2m1x8(b);
+  return lo == hi ? lo : resolve8(lo, hi, u, half, s, o);
+}
+
+__device__ __forceinline__ uint32_t mx_codes8(const float (&x)[8], float inv) {
+  float a[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a[j] = __fmul_rn(x[j], inv);  // exact, or far below the first border
+  return e2m1x8(a);
+}
+
+// 32 bytes that no kernel in flight writes; `wide`: the address is a multiple of
+// 32 (one load), else of 16.  Not volatile: an unrolled loop's loads may all be
+// issued ahead of its stores.
 __device__ __forceinline__ void ld_stream32(const void* p, bool wide, uint4& a, uint4& b) {
   if (wide) {
-    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+    asm("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z),
                    "=r"(b.w)
                  : "l"(p));
@@ -162,6 +183,13 @@ __device__ __forceinline__ void ld_stream32(const void* p, bool wide, uint4& a, 
     a = ld_cached16(p);
     b = ld_cached16(static_cast<const uint8_t*>(p) + 16);
   }
+}
+
+// 32 bytes to a multiple of 32.
+__device__ __forceinline__ void st_global32(void* p, const uint4& a, const uint4& b) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(a.x), "r"(a.y),
+               "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
 }
 
 template <typename T>
@@ -219,19 +247,47 @@ __device__ __forceinline__ void unit_values(const Unit<T>& u, int half, float (&
   }
 }
 
-// Largest of one value per thread over the row's group; every thread of the
-// block takes part.
-__device__ __forceinline__ uint32_t group_max_bits(uint32_t v, int tpr, uint32_t* red) {
+// Wait for the threads of this row's group (tpr <= 32: a warp, nothing to wait
+// for).  A barrier of its own for each group: the rows of a block do not wait
+// for one another.
+__device__ __forceinline__ void group_sync(int tpr) {
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / tpr), "r"(tpr)
+               : "memory");
+}
+
+// Shared words of a block's reductions: a slot per warp for each, written once.
+struct GroupRed {
+  double sum[8];
+  uint32_t top[8];
+};
+
+// Largest of one value per thread over the row's group.
+__device__ __forceinline__ uint32_t group_max_bits(uint32_t v, int tpr, GroupRed& red) {
   v = __reduce_max_sync(0xffffffffu, v);  // a group is whole warps
   if (tpr > 32) {
     const int warp = threadIdx.x >> 5;
     const int wpr = tpr >> 5;
     const int first = warp / wpr * wpr;
-    __syncthreads();  // `red` may still be read from its previous use
-    if ((threadIdx.x & 31) == 0) red[warp] = v;
-    __syncthreads();
-    v = red[first];
-    for (int w = 1; w < wpr; ++w) v = max(v, red[first + w]);
+    if ((threadIdx.x & 31) == 0) red.top[warp] = v;
+    group_sync(tpr);
+    v = red.top[first];
+    for (int w = 1; w < wpr; ++w) v = max(v, red.top[first + w]);
+  }
+  return v;
+}
+
+// Sum of one double per thread over the row's group.
+__device__ __forceinline__ double group_sum(double v, int tpr, GroupRed& red) {
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  if (tpr > 32) {
+    const int warp = threadIdx.x >> 5;
+    const int wpr = tpr >> 5;
+    const int first = warp / wpr * wpr;
+    if ((threadIdx.x & 31) == 0) red.sum[warp] = v;
+    group_sync(tpr);
+    v = red.sum[first];
+    for (int w = 1; w < wpr; ++w) v += red.sum[first + w];
   }
   return v;
 }
@@ -285,52 +341,211 @@ __device__ __forceinline__ uint32_t convert_unit(const Unit<T>& u, uint32_t m_bi
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       unit_values(u, h, v);
-      c[h] = nv_codes8(v, inv, s, rs.o);
+      c[h] = nv_codes8(u, h, v, inv, s, rs.o);
     }
     return byte;
   }
 }
 
-// Store the codes and the scale byte of unit `unit` of `row`.  TM_FP4_MX blocks
-// span two units (adjacent lanes); the even one stores the byte.
-template <int KIND>
-__device__ __forceinline__ void store_unit(const Fp4Params& p, int64_t row, int64_t unit,
-                                           const uint32_t (&c)[2], uint32_t byte) {
-  *reinterpret_cast<uint2*>(p.codes + row * (p.cols / 2) + unit * 8) = make_uint2(c[0], c[1]);
-  if (KIND != kMx || (unit & 1) == 0)
-    p.blocks[fp4_scale_offset(row, KIND == kMx ? unit >> 1 : unit, p.ktiles)] =
-        static_cast<uint8_t>(byte);
+// Where a row's results go: the row's part of every address.
+struct RowOut {
+  uint8_t* codes;
+  uint8_t* blocks;
+};
+
+__device__ __forceinline__ RowOut row_out(const Fp4Params& p, int64_t row) {
+  return RowOut{p.codes + row * (p.cols / 2), p.blocks + fp4_scale_offset(row, 0, p.ktiles)};
 }
 
-// Zero scale byte of a unit that only pads a tile.
+// Scale byte of a unit; TM_FP4_MX blocks span two units (adjacent lanes), the
+// even one stores it.
 template <int KIND>
-__device__ __forceinline__ void store_pad(const Fp4Params& p, int64_t row, int64_t unit) {
+__device__ __forceinline__ void store_scale(const RowOut& out, int unit, uint32_t byte) {
+  const int block = KIND == kMx ? unit >> 1 : unit;
   if (KIND != kMx || (unit & 1) == 0)
-    p.blocks[fp4_scale_offset(row, KIND == kMx ? unit >> 1 : unit, p.ktiles)] = 0;
+    out.blocks[(block >> 2) * 512 + (block & 3)] = static_cast<uint8_t>(byte);
+}
+
+template <int KIND>
+__device__ __forceinline__ void store_unit(const RowOut& out, int unit, const uint32_t (&c)[2],
+                                           uint32_t byte) {
+  *reinterpret_cast<uint2*>(out.codes + unit * 8) = make_uint2(c[0], c[1]);
+  store_scale<KIND>(out, unit, byte);
+}
+
+// ---- adaLN producers on a row held as units of packed bf16 ----
+// The steps of the int8 producers, each rounded to bf16, two values at a time.
+// The bf16x2 multiply and add round the exact result once, which equals the
+// fp32 operation followed by the rounding to bf16: products of two bf16 values
+// are exact in fp32, and a sum either is exact there (24 bits hold two 8-bit
+// significands up to 16 binades apart) or is too far from a bf16 midpoint for
+// the first rounding to matter.
+__device__ __forceinline__ uint32_t bf2_mul(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmul2_rn(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                      *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t bf2_add(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hadd2_rn(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                      *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint64_t bf2_to_f32x2(uint32_t w) {
+  return f32x2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// Word w (0..7) of a unit.
+__device__ __forceinline__ uint32_t& unit_word(Unit<__nv_bfloat16>& u, int w) {
+  return reinterpret_cast<uint32_t*>(u.raw)[w];
+}
+
+// 1 / sqrt(mean of squares + eps) of the row, as the int8 producers compute it:
+// exact fp32 squares added in compensated fp32 chains (TwoSum: every rounding
+// error is kept in a second word), the chains in fp64, then two correctly
+// rounded fp32 steps.
+template <int VPT>
+__device__ __forceinline__ float row_rms_inverse(const Fp4Params& p, Unit<__nv_bfloat16> (&u)[VPT],
+                                                 int tpr, GroupRed& red) {
+  uint64_t sum[2] = {0ull, 0ull}, err[2] = {0ull, 0ull};
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const uint64_t x = bf2_to_f32x2(unit_word(u[i], w));
+      const uint64_t sq = mul_f32x2(x, x);
+      uint64_t &s = sum[w & 1], &e = err[w & 1];
+      const uint64_t t = add_f32x2(s, sq);
+      const uint64_t z = sub_f32x2(t, s);
+      e = add_f32x2(e, add_f32x2(sub_f32x2(s, sub_f32x2(t, z)), sub_f32x2(sq, z)));
+      s = t;
+    }
+  }
+  double ss = 0.0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    float s0, s1, e0, e1;
+    f32x2_split(sum[j], s0, s1);
+    f32x2_split(err[j], e0, e1);
+    ss += (static_cast<double>(s0) + e0) + (static_cast<double>(s1) + e1);
+  }
+  ss = group_sum(ss, tpr, red);
+  const float variance = __double2float_rn(__dmul_rn(ss, p.inv_cols));
+  return rsqrt_two_step_rn(__fadd_rn(variance, p.eps));
+}
+
+// A producer applied to the row's units, in place; also writes the updated
+// residual and the hidden state where there are such outputs.
+template <int VPT, int MODE>
+__device__ __forceinline__ void adaln_units(const Fp4Params& p, Unit<__nv_bfloat16> (&u)[VPT],
+                                            int64_t row, int t, int tpr, int units, bool active,
+                                            bool wide, GroupRed& red) {
+  using U = Unit<__nv_bfloat16>;
+  const int64_t trow = active ? (p.index ? p.index[row] : row) : 0;
+  const auto unit_of = [&](int i) { return t + i * tpr; };
+  const auto load = [&](U& v, const __nv_bfloat16* at, int unit) {
+    v.raw[0] = ld_cached16(at + unit * 16);
+    v.raw[1] = ld_cached16(at + unit * 16 + 8);
+  };
+  const auto store = [&](__nv_bfloat16* at, int unit, const U& v) {
+    uint4* dst = reinterpret_cast<uint4*>(at + (row * p.cols + unit * 16));
+    if (wide) {
+      st_global32(dst, v.raw[0], v.raw[1]);
+    } else {
+      dst[0] = v.raw[0];
+      dst[1] = v.raw[1];
+    }
+  };
+  // per-row tables come from HBM like x: all of them are asked for at once
+  U pre_sc[MODE == kModulateRows ? VPT : 1], pre_sh[MODE == kModulateRows ? VPT : 1];
+  if constexpr (MODE == kModulateRows) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if (active && unit_of(i) < units) {
+        load(pre_sc[i], p.mod_scale + trow * p.table_stride, unit_of(i));
+        load(pre_sh[i], p.shift + trow * p.table_stride, unit_of(i));
+      }
+  }
+  if constexpr (MODE == kResGateRmsModulate) {
+    const __nv_bfloat16* branch = p.branch + row * p.cols;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      if (active && unit_of(i) < units) {
+        U b, g;
+        ld_stream32(branch + unit_of(i) * 16, wide, b.raw[0], b.raw[1]);
+        load(g, p.gate + trow * p.table_stride, unit_of(i));
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+          unit_word(u[i], w) =
+              bf2_add(unit_word(u[i], w), bf2_mul(unit_word(g, w), unit_word(b, w)));
+        store(p.residual_out, unit_of(i), u[i]);
+      }
+    }
+  }
+  uint64_t rinv2 = 0;
+  if constexpr (!modulate_only(MODE)) {
+    const float rinv = row_rms_inverse(p, u, tpr, red);
+    rinv2 = f32x2(rinv, rinv);
+  }
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    if (active && unit_of(i) < units) {
+      U wt, sc, sh;
+      if constexpr (!modulate_only(MODE)) load(wt, p.norm_w, unit_of(i));
+      if constexpr (MODE == kModulateRows) {
+        sc = pre_sc[i];
+        sh = pre_sh[i];
+      } else {
+        load(sc, p.mod_scale + trow * p.table_stride, unit_of(i));
+        load(sh, p.shift + trow * p.table_stride, unit_of(i));
+      }
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        uint32_t x = unit_word(u[i], w);
+        if constexpr (!modulate_only(MODE)) {
+          const uint64_t v =
+              mul_f32x2(mul_f32x2(bf2_to_f32x2(x), rinv2), bf2_to_f32x2(unit_word(wt, w)));
+          float lo, hi;
+          f32x2_split(v, lo, hi);
+          x = pack_bf16x2(lo, hi);
+        }
+        x = bf2_mul(x, bf2_add(0x3f803f80u, unit_word(sc, w)));  // x (1 + scale)
+        unit_word(u[i], w) = bf2_add(x, unit_word(sh, w));
+      }
+      if (p.hidden_out != nullptr) store(p.hidden_out, unit_of(i), u[i]);
+    }
+  }
+}
+
+// Blocks an SM must hold (a cap on registers): the loads of some rows overlap
+// the reductions and the arithmetic of others.
+template <typename T, int VPT, int MODE>
+constexpr int fp4_min_blocks() {
+  if (sizeof(T) == 4) return VPT <= 3 ? 3 : 1;
+  if (MODE == kDynamic || MODE == kModulate) return VPT <= 3 ? 4 : 2;
+  return VPT <= 3 ? 3 : 2;
 }
 
 // A row group per row, the row in registers.  MODE: an adaLN producer, or
 // kDynamic for a plain row.
 template <typename T, int VPT, int MODE, int KIND>
-__global__ void __launch_bounds__(256) quant_fp4_rows_kernel(const Fp4Params p, const bool wide) {
+__global__ void __launch_bounds__(256, (fp4_min_blocks<T, VPT, MODE>())) quant_fp4_rows_kernel(const Fp4Params p, const bool wide) {
   griddep_wait();  // the rows may come from the previous kernel on the stream
   griddep_launch_dependents();
-  __shared__ double red_f64[8];
-  uint32_t* red = reinterpret_cast<uint32_t*>(red_f64);
+  __shared__ GroupRed red;
   const int tpr = 1 << p.tpr_log2;
   const int t = threadIdx.x & (tpr - 1);
   const int64_t row =
       static_cast<int64_t>(blockIdx.x) * (blockDim.x >> p.tpr_log2) + (threadIdx.x >> p.tpr_log2);
   const bool active = row < p.rows;
-  const int64_t units = p.cols / 16;
-  const int64_t pad_units = p.ktiles * (KIND == kMx ? 8 : 4);
+  const int units = static_cast<int>(p.cols / 16);
+  const int pad_units = static_cast<int>(p.ktiles) * (KIND == kMx ? 8 : 4);
   const T* xr = static_cast<const T*>(p.x) + (active ? row : 0) * p.ldx;
   constexpr bool kAdaLN = MODE != kDynamic;
 
   Unit<T> u[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int64_t unit = t + static_cast<int64_t>(i) * tpr;
+    const int unit = t + i * tpr;
     if (active && unit < units)
       load_unit(u[i], xr + unit * 16, wide);
     else
@@ -338,25 +553,7 @@ __global__ void __launch_bounds__(256) quant_fp4_rows_kernel(const Fp4Params p, 
   }
   if constexpr (kAdaLN) {
     static_assert(std::is_same<T, __nv_bfloat16>::value, "adaLN modes are bf16");
-    uint4 raw[2 * VPT], pre_sc[2 * VPT], pre_sh[2 * VPT];
-#pragma unroll
-    for (int i = 0; i < 2 * VPT; ++i) raw[i] = u[i >> 1].raw[i & 1];
-    if constexpr (MODE == kModulateRows) {
-      const int64_t trow = active ? row : 0;
-#pragma unroll
-      for (int i = 0; i < 2 * VPT; ++i) {
-        const int64_t vi = vec_index<true>(t, i, tpr);
-        const bool in = active && vi < 2 * units;
-        const __nv_bfloat16* sc = p.mod_scale + trow * p.table_stride + vi * 8;
-        const __nv_bfloat16* sh = p.shift + trow * p.table_stride + vi * 8;
-        pre_sc[i] = in ? ld_cached16(sc) : make_uint4(0u, 0u, 0u, 0u);
-        pre_sh[i] = in ? ld_cached16(sh) : make_uint4(0u, 0u, 0u, 0u);
-      }
-    }
-    adaln_rows<2 * VPT, MODE, true>(p, raw, pre_sc, pre_sh, row, t, tpr, 2 * units, active,
-                                    red_f64);
-#pragma unroll
-    for (int i = 0; i < 2 * VPT; ++i) u[i >> 1].raw[i & 1] = raw[i];
+    adaln_units<VPT, MODE>(p, u, row, t, tpr, units, active, wide, red);
   }
 
   uint32_t m[VPT];
@@ -376,15 +573,16 @@ __global__ void __launch_bounds__(256) quant_fp4_rows_kernel(const Fp4Params p, 
     rs = given_scale(__ldg(p.static_scale));
   }
   if (row >= p.padded_rows) return;
+  const RowOut out = row_out(p, row);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int64_t unit = t + static_cast<int64_t>(i) * tpr;
+    const int unit = t + i * tpr;
     if (active && unit < units) {
       uint32_t c[2];
       const uint32_t byte = convert_unit<T, KIND>(u[i], m[i], rs, c);
-      store_unit<KIND>(p, row, unit, c, byte);
-    } else if (unit < pad_units) {
-      store_pad<KIND>(p, row, unit);
+      store_unit<KIND>(out, unit, c, byte);
+    } else if (unit < pad_units) {  // blocks that only pad a tile
+      store_scale<KIND>(out, unit, 0u);
     }
   }
 }
@@ -395,19 +593,19 @@ template <typename T, int KIND>
 __global__ void __launch_bounds__(256) quant_fp4_any_kernel(const Fp4Params p) {
   griddep_wait();
   griddep_launch_dependents();
-  __shared__ uint32_t red[8];
+  __shared__ GroupRed red;
   const int64_t row = blockIdx.x;
   const bool active = row < p.rows;
-  const int64_t units = p.cols / 16;
-  const int64_t pad_units = p.ktiles * (KIND == kMx ? 8 : 4);
+  const int units = static_cast<int>(p.cols / 16);
+  const int pad_units = static_cast<int>(p.ktiles) * (KIND == kMx ? 8 : 4);
   const T* xr = static_cast<const T*>(p.x) + (active ? row : 0) * p.ldx;
   RowScale rs{};
   if constexpr (KIND == kNvDynamic) {
     uint32_t top = 0;
     if (active) {
-      for (int64_t unit = threadIdx.x; unit < units; unit += blockDim.x) {
+      for (int unit = threadIdx.x; unit < units; unit += 256) {
         Unit<T> u;
-        load_unit_scalar(u, xr + unit * 16);
+        load_unit_scalar(u, xr + unit * 16ll);
         top = max(top, unit_max_bits(u));
       }
     }
@@ -416,12 +614,13 @@ __global__ void __launch_bounds__(256) quant_fp4_any_kernel(const Fp4Params p) {
   } else if constexpr (KIND == kNvGiven) {
     rs = given_scale(__ldg(p.static_scale));
   }
-  const int64_t lane_units = (pad_units + 255) / 256 * 256;  // whole warps: shuffles below
-  for (int64_t unit = threadIdx.x; unit < lane_units; unit += blockDim.x) {
+  const RowOut out = row_out(p, row);
+  const int lane_units = (pad_units + 255) / 256 * 256;  // whole warps: shuffles below
+  for (int unit = threadIdx.x; unit < lane_units; unit += 256) {
     Unit<T> u;
     const bool in = active && unit < units;
     if (in)
-      load_unit_scalar(u, xr + unit * 16);
+      load_unit_scalar(u, xr + unit * 16ll);
     else
       clear_unit(u);
     uint32_t m = unit_max_bits(u);
@@ -429,9 +628,9 @@ __global__ void __launch_bounds__(256) quant_fp4_any_kernel(const Fp4Params p) {
     if (in) {
       uint32_t c[2];
       const uint32_t byte = convert_unit<T, KIND>(u, m, rs, c);
-      store_unit<KIND>(p, row, unit, c, byte);
-    } else if (unit < pad_units) {
-      store_pad<KIND>(p, row, unit);
+      store_unit<KIND>(out, unit, c, byte);
+    } else if (unit < pad_units) {  // blocks that only pad a tile
+      store_scale<KIND>(out, unit, 0u);
     }
   }
 }
@@ -445,6 +644,7 @@ struct DequantParams {
   bool per_row;
   int64_t rows, cols, ktiles;
   int tpr_log2;
+  bool wide;  // out on a 32-byte boundary (its rows are multiples of 64 bytes)
 };
 
 // Two e2m1 codes -> two values.
@@ -459,24 +659,32 @@ __device__ __forceinline__ float2 e2m1x2_to_f32(uint32_t byte) {
 }
 
 template <typename T>
-__device__ __forceinline__ void store16(T* out, const float (&v)[16]) {
+__device__ __forceinline__ void store16(T* out, const float (&v)[16], bool wide) {
+  uint4 w[sizeof(T)];
+  uint32_t* e = reinterpret_cast<uint32_t*>(w);
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int j = 0; j < 16; j += 4)
-      *reinterpret_cast<float4*>(out + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    for (int j = 0; j < 16; ++j) e[j] = __float_as_uint(v[j]);
   } else {
-    uint32_t w[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+        e[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
       } else {
         const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-        w[j] = *reinterpret_cast<const uint32_t*>(&h);
+        e[j] = *reinterpret_cast<const uint32_t*>(&h);
       }
     }
-    reinterpret_cast<uint4*>(out)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    reinterpret_cast<uint4*>(out)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+#pragma unroll
+  for (int j = 0; j < static_cast<int>(sizeof(T)); j += 2) {
+    uint4* dst = reinterpret_cast<uint4*>(out) + j;
+    if (wide) {
+      st_global32(dst, w[j], w[j + 1]);
+    } else {
+      dst[0] = w[j];
+      dst[1] = w[j + 1];
+    }
   }
 }
 
@@ -491,14 +699,16 @@ __global__ void __launch_bounds__(256) dequant_fp4_kernel(const DequantParams p)
   const int64_t row =
       static_cast<int64_t>(blockIdx.x) * (blockDim.x >> p.tpr_log2) + (threadIdx.x >> p.tpr_log2);
   if (row >= p.rows) return;
-  const int64_t units = p.cols / 16;
+  const int units = static_cast<int>(p.cols / 16);
+  const uint8_t* blocks = p.blocks + fp4_scale_offset(row, 0, p.ktiles);
+  const uint2* codes = reinterpret_cast<const uint2*>(p.codes + row * (p.cols / 2));
   const float o = p.scales == nullptr ? 1.0f : __ldg(p.scales + (p.per_row ? row : 0));
   T* out = static_cast<T*>(p.out) + row * p.cols;
 #pragma unroll 4
-  for (int64_t unit = t; unit < units; unit += tpr) {
-    const uint2 c = __ldg(reinterpret_cast<const uint2*>(p.codes + row * (p.cols / 2)) + unit);
-    const uint32_t byte =
-        __ldg(p.blocks + fp4_scale_offset(row, FORMAT == TM_FP4_MX ? unit >> 1 : unit, p.ktiles));
+  for (int unit = t; unit < units; unit += tpr) {
+    const uint2 c = __ldg(codes + unit);
+    const int block = FORMAT == TM_FP4_MX ? unit >> 1 : unit;
+    const uint32_t byte = __ldg(blocks + (block >> 2) * 512 + (block & 3));
     float s;
     if constexpr (FORMAT == TM_FP4_MX)  // 2^(byte - 127); 0 is the subnormal 2^-127, 255 NaN
       s = __uint_as_float(byte == 255u ? 0x7fffffffu : byte == 0u ? 0x00400000u : byte << 23);
@@ -511,7 +721,7 @@ __global__ void __launch_bounds__(256) dequant_fp4_kernel(const DequantParams p)
       v[2 * j] = __fmul_rn(__fmul_rn(q.x, s), o);
       v[2 * j + 1] = __fmul_rn(__fmul_rn(q.y, s), o);
     }
-    store16(out + unit * 16, v);
+    store16(out + unit * 16, v, p.wide);
   }
 }
 
@@ -600,6 +810,7 @@ int launch_typed(const Fp4Params& p, int dtype, cudaStream_t stream) {
 int set_geometry(Fp4Params& p, int format, int64_t rows, int64_t cols, int64_t ld) {
   if (format != TM_FP4_NV && format != TM_FP4_MX) return TM_ERR_UNSUPPORTED;
   if (rows < 0 || cols <= 0 || cols % 32 != 0 || ld < cols) return TM_ERR_SHAPE;
+  if (cols > (1ll << 30)) return TM_ERR_TOO_LARGE;  // positions within a row are 32-bit
   p.rows = rows;
   p.cols = cols;
   p.ldx = ld;
@@ -616,15 +827,11 @@ int launch_adaln(Fp4Params p, int format, cudaStream_t stream) {
       (MODE == kResGateRmsModulate &&
        (!aligned16(p.branch) || !aligned16(p.gate) || !aligned16(p.residual_out))))
     return TM_ERR_ALIGNMENT;
-  // as for the int8 producers: one warp a row in the RMSNorm modes while the
-  // row fits (widths up to 3072)
-  int tpr_log2 = 5, vpt = 0;
-  const int64_t units = p.cols / 16;
-  if (!modulate_only(MODE) && units <= 32 * 6)
-    vpt = static_cast<int>((units + 31) / 32);
-  else if (!pick_fp4_layout<__nv_bfloat16>(units, &tpr_log2, &vpt))
-    return TM_ERR_TOO_LARGE;
-  const bool wide = multiple_of(p.x, p.ldx * 2, 32);
+  int tpr_log2 = 0, vpt = 0;
+  if (!pick_fp4_layout<__nv_bfloat16>(p.cols / 16, &tpr_log2, &vpt)) return TM_ERR_TOO_LARGE;
+  // rows are multiples of 64 bytes: 32-byte accesses wherever the tensors start on one
+  const auto on32 = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 32 == 0; };
+  const bool wide = on32(p.x) && on32(p.hidden_out) && on32(p.branch) && on32(p.residual_out);
   return format == TM_FP4_MX
              ? launch_rows<__nv_bfloat16, MODE, kMx>(p, tpr_log2, vpt, wide, stream)
              : launch_rows<__nv_bfloat16, MODE, kNvDynamic>(p, tpr_log2, vpt, wide, stream);
@@ -719,6 +926,7 @@ int tm_dequantize_fp4(void* out, int out_dtype, const uint8_t* q, const uint8_t*
   p.rows = rows;
   p.cols = cols;
   p.ktiles = g.ktiles;
+  p.wide = reinterpret_cast<uintptr_t>(out) % 32 == 0;
   p.tpr_log2 = 5;
   while (p.tpr_log2 < 8 && (cols / 16) > (4ll << p.tpr_log2)) ++p.tpr_log2;
   const cudaStream_t st = tmw::as_stream(stream);

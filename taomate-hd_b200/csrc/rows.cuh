@@ -1,6 +1,6 @@
 // Row-group building blocks shared by the quantisation kernels (int8 and
-// 4-bit): streaming loads, reductions over the threads that own a row, and
-// the adaLN producers that rewrite a row held as packed bf16.
+// 4-bit): parameters, streaming loads, reductions over the threads that own a
+// row, and the correctly rounded reciprocal square root of the RMSNorm.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -232,134 +232,6 @@ __device__ __forceinline__ float rsqrt_two_step_rn(float v) {
     q = f32_next_down(q);
   }
   return q;
-}
-
-// Index of thread t's i-th 16-byte vector of a row: strided by the group's
-// width, or (kPaired) in adjacent pairs, so that a thread holds 32 contiguous
-// bytes.
-template <bool kPaired>
-__device__ __forceinline__ int64_t vec_index(int t, int i, int tpr) {
-  if constexpr (kPaired)
-    return 2 * (t + static_cast<int64_t>(i >> 1) * tpr) + (i & 1);
-  else
-    return t + static_cast<int64_t>(i) * tpr;
-}
-
-// adaLN producers on a row held as packed bf16 (8 values per uint4; every
-// intermediate below is rounded to bf16, so the packed form loses nothing):
-//   kResGateRmsModulate: x = bf16(x + bf16(gate[t] * branch)) -> residual_out
-//   kRmsModulate (and the above): x = bf16(x * rsqrt(mean(x^2) + eps) * w)
-//   all three:          h = bf16(bf16(x * bf16(1 + scale[t])) + shift[t])
-// h replaces the row in `raw` (and goes to hidden_out when requested); the
-// caller quantises it as a plain bf16 row.  Table loads are plain read-only
-// loads the compiler can issue ahead of the stores.
-//
-// kPaired: the row's vectors are dealt out in adjacent pairs (vec_index).
-template <int VPT, int MODE, bool kPaired = false>
-__device__ __forceinline__ void adaln_rows(const QuantParams& p, uint4 (&raw)[VPT],
-                                           const uint4 (&pre_sc)[VPT],
-                                           const uint4 (&pre_sh)[VPT], int64_t row,
-                                           int t, int tpr, int64_t nvec, bool active,
-                                           double* red) {
-  constexpr int E = 8;
-  const int64_t trow = active ? (p.index ? p.index[row] : row) : 0;
-  if constexpr (MODE == kResGateRmsModulate) {
-    const __nv_bfloat16* gate_row = p.gate + trow * p.table_stride;
-    const __nv_bfloat16* branch_row = p.branch + row * p.cols;
-    uint4 gr[VPT], br[VPT];
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int64_t vi = vec_index<kPaired>(t, i, tpr);
-      if (active && vi < nvec) {
-        gr[i] = ld_cached16(gate_row + vi * E);
-        br[i] = ld_nc16(branch_row + vi * E);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int64_t vi = vec_index<kPaired>(t, i, tpr);
-      if (active && vi < nvec) {
-        uint32_t* xw = reinterpret_cast<uint32_t*>(&raw[i]);
-        const uint32_t* gw = reinterpret_cast<const uint32_t*>(&gr[i]);
-        const uint32_t* bw = reinterpret_cast<const uint32_t*>(&br[i]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 x = unpack_bf16x2(xw[j]), g = unpack_bf16x2(gw[j]),
-                       b = unpack_bf16x2(bw[j]);
-          xw[j] = pack_bf16x2(round_bf16(__fadd_rn(x.x, round_bf16(__fmul_rn(g.x, b.x)))),
-                              round_bf16(__fadd_rn(x.y, round_bf16(__fmul_rn(g.y, b.y)))));
-        }
-        *reinterpret_cast<uint4*>(p.residual_out + row * p.cols + vi * E) = raw[i];
-      }
-    }
-  }
-  float rinv = 0.f;
-  if constexpr (MODE == kRmsModulate || MODE == kResGateRmsModulate) {
-    // rinv = fp32(1 / fp32(sqrt(fp32(mean(x^2)) + eps))) with every step
-    // correctly rounded, as the reference kernel's arithmetic is restated by
-    // its oracle (a float64 mean, then IEEE fp32 add, sqrt and division; no
-    // approximate rsqrt).  The square of a bf16 value is exact in fp32; each
-    // thread sums its squares in four compensated fp32 chains (TwoSum: the
-    // rounding error of every add is kept in a second word), so s + c carries
-    // the sum to about 2^-40 relative; the pairs are then added in fp64.
-    float cs[4] = {0.f, 0.f, 0.f, 0.f}, cc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const uint32_t* xw = reinterpret_cast<const uint32_t*>(&raw[i]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 x = unpack_bf16x2(xw[j]);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float v = e ? x.y : x.x;
-          const float sq = __fmul_rn(v, v);
-          const float t = __fadd_rn(cs[j], sq);
-          const float z = __fsub_rn(t, cs[j]);
-          cc[j] = __fadd_rn(cc[j], __fadd_rn(__fsub_rn(cs[j], __fsub_rn(t, z)), __fsub_rn(sq, z)));
-          cs[j] = t;
-        }
-      }
-    }
-    double ss = 0.0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      ss = __dadd_rn(ss, __dadd_rn(static_cast<double>(cs[j]), static_cast<double>(cc[j])));
-    ss = group_sum_f64(ss, tpr, red);
-    const float variance = __double2float_rn(__dmul_rn(ss, p.inv_cols));
-    rinv = rsqrt_two_step_rn(__fadd_rn(variance, p.eps));
-  }
-  const __nv_bfloat16* sc_row = p.mod_scale + trow * p.table_stride;
-  const __nv_bfloat16* sh_row = p.shift + trow * p.table_stride;
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int64_t vi = vec_index<kPaired>(t, i, tpr);
-    if (active && vi < nvec) {
-      uint4 wr = make_uint4(0u, 0u, 0u, 0u);
-      if constexpr (!modulate_only(MODE)) wr = ld_cached16(p.norm_w + vi * E);
-      // per-row tables were loaded together with x
-      const uint4 scr = MODE == kModulateRows ? pre_sc[i] : ld_cached16(sc_row + vi * E);
-      const uint4 shr = MODE == kModulateRows ? pre_sh[i] : ld_cached16(sh_row + vi * E);
-      uint32_t* xw = reinterpret_cast<uint32_t*>(&raw[i]);
-      const uint32_t* ww = reinterpret_cast<const uint32_t*>(&wr);
-      const uint32_t* cw = reinterpret_cast<const uint32_t*>(&scr);
-      const uint32_t* hw = reinterpret_cast<const uint32_t*>(&shr);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float2 x = unpack_bf16x2(xw[j]);
-        if constexpr (!modulate_only(MODE)) {
-          const float2 w = unpack_bf16x2(ww[j]);
-          x.x = round_bf16(__fmul_rn(__fmul_rn(x.x, rinv), w.x));
-          x.y = round_bf16(__fmul_rn(__fmul_rn(x.y, rinv), w.y));
-        }
-        const float2 c = unpack_bf16x2(cw[j]), sh = unpack_bf16x2(hw[j]);
-        const float m0 = round_bf16(__fmul_rn(x.x, round_bf16(__fadd_rn(1.0f, c.x))));
-        const float m1 = round_bf16(__fmul_rn(x.y, round_bf16(__fadd_rn(1.0f, c.y))));
-        xw[j] = pack_bf16x2(__fadd_rn(m0, sh.x), __fadd_rn(m1, sh.y));
-      }
-      if (p.hidden_out != nullptr)
-        *reinterpret_cast<uint4*>(p.hidden_out + row * p.cols + vi * E) = raw[i];
-    }
-  }
 }
 
 }  // namespace
