@@ -86,7 +86,7 @@ __device__ __forceinline__ uint8_t* align1k(uint8_t* p) {
 }
 
 // ====================================================================== small
-constexpr int kSmallThreads = 192;  // producer, MMA, four epilogue warps
+constexpr int kSmallThreads = 320;  // producer, MMA, eight epilogue warps
 constexpr int kMaxStages = 8;
 
 template <int TOK, int FORMAT>
@@ -98,7 +98,7 @@ struct SmallLayout {
   static constexpr int kStageBytes = kWBytes + kXBytes + 2 * S::kBytes;
   static_assert(kStageBytes % 1024 == 0, "stages stay aligned");
   static constexpr int kReduceBytes = kTileRows * TOK * 4;
-  static constexpr int kBarBytes = 256;
+  static constexpr int kBarBytes = 256 + kTileRows * 4;  // and the tokens' scales
   static constexpr int total(int stages, int splits) {
     return 1024 + stages * kStageBytes + kBarBytes + (splits > 1 ? kReduceBytes : 0);
   }
@@ -132,8 +132,8 @@ __device__ __forceinline__ SmallBars small_bars(uint8_t* base) {
   return b;
 }
 
-__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+__device__ __forceinline__ void st_cluster_f32x2(uint32_t addr, float a, float b) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(a), "f"(b) : "memory");
 }
 
 // What a lane of an epilogue warp keeps: its weight row's constants.
@@ -152,19 +152,16 @@ __device__ __forceinline__ RowConsts row_consts(const Fp4Args& g, int n) {
   return c;
 }
 
-// Finish and store the sums of tokens m and m + 1, a weight row per lane (the
-// lanes of a warp are 32 consecutive output columns).  Neighbouring lanes
-// exchange a value, so that each stores two columns of one token.  `tokens`: 2,
-// or 1 when there is no second token.  Called by the whole warp.
+// Finish and store the sums of two tokens, a weight row per lane (the lanes of a
+// warp are 32 consecutive output columns).  Neighbouring lanes exchange a value,
+// so that each stores two columns of one token.  `second`: there is a second
+// token.  sa: the tokens' scales.  Called by the whole warp.
 template <int EPI, typename OutT>
 __device__ __forceinline__ void store_tokens(const Fp4Args& g, const RowConsts& c, int64_t m,
-                                             int tokens, float acc0, float acc1) {
+                                             bool second, float2 sa, float acc0, float acc1) {
   const int lane = threadIdx.x & 31;
-  const int64_t m1 = tokens > 1 ? m + 1 : m;
-  const float sa0 = g.sa == nullptr ? 1.f : __ldg(g.sa + (g.sa_per_row ? m : 0));
-  const float sa1 = g.sa == nullptr ? 1.f : __ldg(g.sa + (g.sa_per_row ? m1 : 0));
-  float y0 = __fmaf_rn(sa0, __fmul_rn(c.sb, acc0), c.bias);
-  float y1 = __fmaf_rn(sa1, __fmul_rn(c.sb, acc1), c.bias);
+  float y0 = __fmaf_rn(sa.x, __fmul_rn(c.sb, acc0), c.bias);
+  float y1 = __fmaf_rn(sa.y, __fmul_rn(c.sb, acc1), c.bias);
   int col = c.n;
   bool in = c.n < g.N;
   if constexpr (EPI == TM_EPI_GELU_TANH) {
@@ -181,40 +178,79 @@ __device__ __forceinline__ void store_tokens(const Fp4Args& g, const RowConsts& 
   }
   const bool odd = lane & 1;  // odd lanes take the second token
   const float got = __shfl_xor_sync(0xffffffffu, odd ? y0 : y1, 1);
-  if (in && (!odd || tokens > 1)) {
-    OutT* dst = static_cast<OutT*>(g.out) + (odd ? m1 : m) * g.ldo + (col & ~1);
+  if (in && (!odd || second)) {
+    OutT* dst = static_cast<OutT*>(g.out) + (m + odd) * g.ldo + (col & ~1);
     *reinterpret_cast<uint32_t*>(dst) = odd ? pack2<OutT>(got, y1) : pack2<OutT>(y0, got);
   }
 }
 
+// The epilogue warps' work, in loops short enough to be fetched quickly: these
+// kernels run their code once.  Warp half h (0, 1) takes every other group of
+// eight tokens, or every other pair.
 template <int EPI, typename OutT>
-__device__ __forceinline__ void store_tile(const Fp4Args& g, const RowConsts& c, uint32_t t_row,
-                                           int64_t m0, int tokens) {
+__device__ __forceinline__ void store_tile(const Fp4Args& g, const RowConsts& c, const float* sa,
+                                           uint32_t t_row, int64_t m0, int tokens, int h) {
 #pragma unroll 1
-  for (int t = 0; t < tokens; t += 32) {
-    uint32_t r[32];
-    tmem_ld_32x32b_x32(t_row + t, r);
+  for (int t = 8 * h; t < tokens; t += 16) {
+    uint32_t r[8];
+    tmem_ld_32x32b_x8(t_row + t, r);
     tmem_ld_wait();
 #pragma unroll
-    for (int j = 0; j < 32; j += 2)
+    for (int j = 0; j < 8; j += 2)
       if (t + j < tokens)  // the same for the whole warp
-        store_tokens<EPI, OutT>(g, c, m0 + t + j, tokens - t - j, __uint_as_float(r[j]),
-                                __uint_as_float(r[j + 1]));
+        store_tokens<EPI, OutT>(g, c, m0 + t + j, t + j + 1 < tokens,
+                                *reinterpret_cast<const float2*>(sa + t + j),
+                                __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
   }
 }
 
-// The sums of this CTA's tokens, [slice][token][weight row], added in slice order.
-template <int EPI, typename OutT>
-__device__ __forceinline__ void store_reduced(const Fp4Args& g, const RowConsts& c,
-                                              const float* sums, int splits, int per, int64_t m0,
-                                              int tokens) {
-  for (int t = 0; t < tokens; t += 2) {
-    float a0 = 0.f, a1 = 0.f;
-    for (int s = 0; s < splits; ++s) {
-      a0 += sums[(s * per + t) * kTileRows];
-      if (t + 1 < tokens) a1 += sums[(s * per + t + 1) * kTileRows];
+// Pairs of tokens are dealt out to the slices of the cluster: pair p is finished
+// by slice p % splits, its sums at sums[slice][p / splits][weight row].
+constexpr int kMaxSplits = 8;
+
+__device__ __forceinline__ void send_sums(float2* sums, uint32_t t_row, int row, int tokens,
+                                          int slice, int splits, int log_splits, int h, bool ok) {
+  const int pairs = ((tokens + 1) / 2 + splits - 1) >> log_splits;  // of one slice
+  const uint32_t mine = smem_u32(sums + slice * pairs * kTileRows + row);
+#pragma unroll 1
+  for (int t = 8 * h; t < tokens; t += 16) {
+    uint32_t r[8];
+    tmem_ld_32x32b_x8(t_row + t, r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const int p = (t + j) >> 1;
+      const uint32_t at = mine + (p >> log_splits) * (kTileRows * 8);
+      const float nan = __int_as_float(0x7fffffff);
+      if (t + j < tokens)
+        st_cluster_f32x2(map_to_cta(at, p & (splits - 1)), ok ? __uint_as_float(r[j]) : nan,
+                         ok ? __uint_as_float(r[j + 1]) : nan);
     }
-    store_tokens<EPI, OutT>(g, c, m0 + t, tokens - t, a0, a1);
+  }
+}
+
+template <int EPI, typename OutT>
+__device__ __forceinline__ void store_reduced(const Fp4Args& g, const RowConsts& c, const float* sa,
+                                              const float2* sums, int row, int64_t m0, int tokens,
+                                              int slice, int splits, int log_splits, int h) {
+  const int all = (tokens + 1) / 2;
+  const int pairs = (all + splits - 1) >> log_splits;
+#pragma unroll 1
+  for (int l = h; l < pairs; l += 2) {
+    const int p = (l << log_splits) + slice;
+    if (p >= all) break;
+    float2 part[kMaxSplits];
+#pragma unroll
+    for (int s = 0; s < kMaxSplits; ++s)
+      part[s] = s < splits ? sums[(s * pairs + l) * kTileRows + row] : make_float2(0.f, 0.f);
+    float a0 = 0.f, a1 = 0.f;
+#pragma unroll
+    for (int s = 0; s < kMaxSplits; ++s) {  // in slice order; the absent ones add 0
+      a0 += part[s].x;
+      a1 += part[s].y;
+    }
+    store_tokens<EPI, OutT>(g, c, m0 + 2 * p, 2 * p + 1 < tokens,
+                            *reinterpret_cast<const float2*>(sa + 2 * p), a0, a1);
   }
 }
 
@@ -230,7 +266,8 @@ __global__ void __launch_bounds__(kSmallThreads)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1k(smem_raw);
   const SmallBars bar = small_bars(smem + g.stages * L::kStageBytes);
-  float* reduce = reinterpret_cast<float*>(smem + g.stages * L::kStageBytes + L::kBarBytes);
+  float* token_sa = reinterpret_cast<float*>(smem + g.stages * L::kStageBytes + 256);
+  float2* sums = reinterpret_cast<float2*>(smem + g.stages * L::kStageBytes + L::kBarBytes);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -255,14 +292,6 @@ __global__ void __launch_bounds__(kSmallThreads)
     tma_prefetch_desc(&tm_x);
     tma_prefetch_desc(&tm_ws);
     tma_prefetch_desc(&tm_xs);
-    // With one token tile the weight is read once: ask for this slice of it
-    // while the previous kernel on the stream still runs (an L2 prefetch has
-    // no effect on what is read later, whoever writes the weight).
-    if (g.num_m == 1)
-      for (int kb = kb0; kb < kb1; ++kb) {
-        tma_prefetch_l2_2d(&tm_w, kb * kRowBytes, nb * kTileRows);
-        tma_prefetch_l2_2d(&tm_ws, kb * (S::kBytes / 8), nb);
-      }
   }
   if (warp == 1) {
     tmem_alloc(bar.tmem_slot, tmem_cols);
@@ -275,6 +304,15 @@ __global__ void __launch_bounds__(kSmallThreads)
     __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *bar.tmem_slot;
+  // With one token tile the weight is read once: ask for this slice of it while
+  // the previous kernel on the stream still runs (an L2 prefetch has no effect
+  // on what is read later, whoever writes the weight).
+  if (threadIdx.x == 64 && g.num_m == 1) {
+    for (int kb = kb0; kb < kb1; ++kb) {
+      tma_prefetch_l2_2d(&tm_w, kb * kRowBytes, nb * kTileRows);
+      tma_prefetch_l2_2d(&tm_ws, kb * (S::kBytes / 8), nb);
+    }
+  }
   griddep_wait();
   griddep_launch_dependents();
 
@@ -375,70 +413,45 @@ __global__ void __launch_bounds__(kSmallThreads)
     }
     __syncwarp();
   } else {
-    const int q = warp & 3;
-    const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+    const int h = (warp - 2) >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t t_row = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const int64_t m0 = static_cast<int64_t>(mb) * TOK;
     const int tokens = static_cast<int>(min(static_cast<int64_t>(TOK), g.M - m0));
-    const RowConsts c = row_consts<OutT>(g, nb * kTileRows + q * 32 + lane);
+    const RowConsts c = row_consts<OutT>(g, nb * kTileRows + row);
+    if (threadIdx.x - 64 < TOK) {
+      const int t = threadIdx.x - 64;
+      token_sa[t] = g.sa == nullptr || t >= tokens ? 1.f : __ldg(g.sa + (g.sa_per_row ? m0 + t : 0));
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");  // the epilogue warps: token_sa is complete
     const bool ok = mbar_wait_warp(bar.acc, 0, bar.abort_flag, g.status);
     tc_fence_after();
-    if (splits == 1) {
-      if (ok) {
-        if (g.epilogue & TM_EPI_GELU_TANH)
-          store_tile<TM_EPI_GELU_TANH, OutT>(g, c, t_row, m0, tokens);
-        else if (g.epilogue & TM_EPI_SWIGLU)
-          store_tile<TM_EPI_SWIGLU, OutT>(g, c, t_row, m0, tokens);
-        else
-          store_tile<0, OutT>(g, c, t_row, m0, tokens);
-      }
-    } else {
-      // Slice j of the cluster finishes tokens [j, j + 1) * per: send it this
-      // slice's sums of those tokens.
-      const int per = (tokens + splits - 1) / splits;
-      const uint32_t mine = smem_u32(reduce) + (slice * per * kTileRows + q * 32 + lane) * 4;
-#pragma unroll 1
-      for (int t = 0; t < tokens; t += 32) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(t_row + t, r);
-        tmem_ld_wait();
-        int to = t / per, at = t - to * per;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          if (t + j < tokens) {
-            st_cluster_f32(map_to_cta(mine + at * kTileRows * 4, to),
-                           ok ? __uint_as_float(r[j]) : __int_as_float(0x7fffffff));
-            if (++at == per) {
-              at = 0;
-              ++to;
-            }
-          }
-        }
-      }
+    const int log_splits = 31 - __clz(splits);
+    if (splits > 1) {
+      send_sums(sums, t_row, row, tokens, slice, splits, log_splits, h, ok);
+      tc_fence_before();
+      cluster_sync();  // every slice's sums have arrived
+      if (g.epilogue & TM_EPI_GELU_TANH)
+        store_reduced<TM_EPI_GELU_TANH, OutT>(g, c, token_sa, sums, row, m0, tokens, slice, splits,
+                                              log_splits, h);
+      else if (g.epilogue & TM_EPI_SWIGLU)
+        store_reduced<TM_EPI_SWIGLU, OutT>(g, c, token_sa, sums, row, m0, tokens, slice, splits,
+                                           log_splits, h);
+      else
+        store_reduced<0, OutT>(g, c, token_sa, sums, row, m0, tokens, slice, splits, log_splits, h);
+    } else if (ok) {
+      if (g.epilogue & TM_EPI_GELU_TANH)
+        store_tile<TM_EPI_GELU_TANH, OutT>(g, c, token_sa, t_row, m0, tokens, h);
+      else if (g.epilogue & TM_EPI_SWIGLU)
+        store_tile<TM_EPI_SWIGLU, OutT>(g, c, token_sa, t_row, m0, tokens, h);
+      else
+        store_tile<0, OutT>(g, c, token_sa, t_row, m0, tokens, h);
     }
   }
 
   tc_fence_before();
-  if (splits > 1) {
-    cluster_sync();  // every slice's sums have arrived
-    if (warp >= 2) {
-      const int row = (warp & 3) * 32 + lane;
-      const RowConsts c = row_consts<OutT>(g, nb * kTileRows + row);
-      const int64_t m0 = static_cast<int64_t>(mb) * TOK;
-      const int tokens = static_cast<int>(min(static_cast<int64_t>(TOK), g.M - m0));
-      const int per = (tokens + splits - 1) / splits;
-      const int mine = min(per, tokens - slice * per);  // <= 0: other slices finish them all
-      const float* sums = reduce + row;
-      const int64_t m = m0 + slice * per;
-      if (g.epilogue & TM_EPI_GELU_TANH)
-        store_reduced<TM_EPI_GELU_TANH, OutT>(g, c, sums, splits, per, m, mine);
-      else if (g.epilogue & TM_EPI_SWIGLU)
-        store_reduced<TM_EPI_SWIGLU, OutT>(g, c, sums, splits, per, m, mine);
-      else
-        store_reduced<0, OutT>(g, c, sums, splits, per, m, mine);
-    }
-  } else {
-    __syncthreads();
-  }
+  if (splits > 1 && warp < 2) cluster_sync();  // the epilogue warps' barrier is for every thread
+  __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, tmem_cols);
@@ -449,7 +462,6 @@ __global__ void __launch_bounds__(kSmallThreads)
 constexpr int kPairThreads = 320;  // producer, MMA, eight epilogue warps
 constexpr int kPairEpiWarps = 8;
 constexpr int kPairRows = 256;     // tokens, and weight rows, of a tile
-constexpr int kPairStages = 5;
 // per epilogue warp: 128 column scales and 128 bias values
 constexpr int kPairBiasCache = 512;
 constexpr int kPairRegion = 768;
@@ -458,14 +470,15 @@ constexpr int kPairRegion = 768;
 // again when its shared memory has been refilled, hence after its MMAs.
 constexpr uint32_t kScaleCol = 256;
 constexpr int kTileCols = 12;
-static_assert(kScaleCol + kPairStages * 4 * kTileCols <= 512, "TMEM columns");
 
 template <int FORMAT>
 struct PairLayout {
   using S = ScaleGeom<FORMAT>;
   static constexpr int kHalfBytes = 128 * kRowBytes;
   static constexpr int kStageBytes = 2 * kHalfBytes + 3 * S::kBytes;  // per CTA
-  static constexpr int kBarOffset = kPairStages * kStageBytes;
+  static constexpr int kStages = FORMAT == TM_FP4_NV ? 5 : 6;
+  static_assert(kScaleCol + kStages * S::kTiles * kTileCols <= 512, "TMEM columns");
+  static constexpr int kBarOffset = kStages * kStageBytes;
   static constexpr int kEpiOffset = kBarOffset + 256;
   static constexpr int kTotal = kEpiOffset + kPairEpiWarps * kPairRegion + 1024;
   static_assert(kStageBytes % 1024 == 0, "stages stay aligned");
@@ -484,8 +497,8 @@ struct PairBars {
 __device__ __forceinline__ PairBars pair_bars(uint8_t* base) {
   PairBars b;
   b.full = reinterpret_cast<uint64_t*>(base);
-  b.empty = b.full + kPairStages;
-  b.acc_full = b.empty + kPairStages;
+  b.empty = b.full + kMaxStages;
+  b.acc_full = b.empty + kMaxStages;
   b.acc_free = b.acc_full + 1;
   b.tmem_slot = reinterpret_cast<uint32_t*>(b.acc_free + 1);
   b.abort_flag = reinterpret_cast<volatile int*>(b.tmem_slot + 1);
@@ -619,7 +632,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   const int pairs = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kPairStages; ++s) {
+    for (int s = 0; s < L::kStages; ++s) {
       mbar_init(&bar.full[s], 1);
       mbar_init(&bar.empty[s], 1);
     }
@@ -675,7 +688,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         __syncwarp();
         issued_mask |= 1u << stage;
         issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
-        if (++stage == kPairStages) {
+        if (++stage == L::kStages) {
           stage = 0;
           phase ^= 1u;
         }
@@ -684,7 +697,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     if (lane == 0) {
       if (!ok) {
         if (leader) {
-          for (int s = 0; s < kPairStages; ++s)
+          for (int s = 0; s < L::kStages; ++s)
             if (issued_mask & (1u << s))
               mbar_wait_drain(&bar.full[s], (issued_parity >> s) & 1u, g.status);
         } else {
@@ -756,7 +769,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           }
           __syncwarp();
           issued_any = true;
-          if (++stage == kPairStages) {
+          if (++stage == L::kStages) {
             stage = 0;
             phase ^= 1u;
           }
@@ -765,7 +778,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         __syncwarp();
       }
       if (!ok && issued_any) {  // the last commit: the tensor pipe has drained
-        const int last = stage == 0 ? kPairStages - 1 : stage - 1;
+        const int last = stage == 0 ? L::kStages - 1 : stage - 1;
         mbar_wait_drain(&bar.empty[last], stage == 0 ? (phase ^ 1u) : phase, g.status);
       }
     }
@@ -988,11 +1001,30 @@ struct Fp4Choice {
   int splits;
 };
 
+// Measured on a B200 (back to back, us): one wave of 128 x 128 tiles is ahead of
+// the pair kernel (512 x 3072 x 3072: 8.2 against 10.1; 1003 x 1160 x 1376: 7.6
+// against 9.5), two waves are behind it (1024 x 3072 x 3072: 11.0 against 10.5;
+// 512 x 12288 x 3072: 20.2 against 16.0), so more than 128 tokens take the small
+// kernel only while its tiles fit the SMs at once.  Up to 128 tokens the weight is
+// read once either way, by twice the CTAs (128 x 12288 x 3072: 9.2 against 10.5).
+//
+// Slices of K: about 0.2 us a k-block, against 0.7 us and what grows with the
+// slices and tokens for the partial sums; only while every slice has an SM of its
+// own (1 x 3072 x 12288: 12.4, 7.6, 6.2 us with 1, 2, 4 slices; 48 x 3072 x 12288
+// mxfp4: 12.7, 9.1, 7.2; 256 x 3072 x 3072: 7.8, 8.9, 13.8).
 Fp4Choice pick_fp4(int64_t m, int64_t n, int kblocks, const Fp4Device& dev) {
-  if (m > 64 && dev.max_pairs > 0) return Fp4Choice{kPairTile, 1};
   Fp4Choice c{m <= 32 ? 32 : m <= 64 ? 64 : 128, 1};
   const int64_t tiles = (m + c.tile - 1) / c.tile * ((n + kTileRows - 1) / kTileRows);
-  while (c.splits < 8 && tiles * c.splits < dev.sms / 2 && kblocks >= 4 * c.splits) c.splits *= 2;
+  if (m > 128 && tiles > dev.sms && dev.max_pairs > 0) return Fp4Choice{kPairTile, 1};
+  const double tokens = static_cast<double>(m < c.tile ? m : c.tile);
+  double best = 0.21 * kblocks;
+  for (int s = 2; s <= kMaxSplits && s <= kblocks && tiles * s <= dev.sms; s *= 2) {
+    const double t = 0.21 * ((kblocks + s - 1) / s) + 0.7 + 0.005 * tokens + 0.1 * s;
+    if (t < best) {
+      best = t;
+      c.splits = s;
+    }
+  }
   return c;
 }
 
