@@ -154,11 +154,12 @@ __device__ __forceinline__ RowConsts row_consts(const Fp4Args& g, int n) {
 
 // Finish and store the sums of two tokens, a weight row per lane (the lanes of a
 // warp are 32 consecutive output columns).  Neighbouring lanes exchange a value,
-// so that each stores two columns of one token.  `second`: there is a second
-// token.  sa: the tokens' scales.  Called by the whole warp.
+// so that each stores two columns of one token.  `left`: tokens from the first
+// on (the stores alone depend on it, so the arithmetic of several pairs
+// overlaps).  sa: the tokens' scales.  Called by the whole warp.
 template <int EPI, typename OutT>
 __device__ __forceinline__ void store_tokens(const Fp4Args& g, const RowConsts& c, int64_t m,
-                                             bool second, float2 sa, float acc0, float acc1) {
+                                             int left, float2 sa, float acc0, float acc1) {
   const int lane = threadIdx.x & 31;
   float y0 = __fmaf_rn(sa.x, __fmul_rn(c.sb, acc0), c.bias);
   float y1 = __fmaf_rn(sa.y, __fmul_rn(c.sb, acc1), c.bias);
@@ -176,9 +177,9 @@ __device__ __forceinline__ void store_tokens(const Fp4Args& g, const RowConsts& 
     col = (c.n >> 5) * 16 + (c.n & 15);
     in = in && lane < 16;
   }
-  const bool odd = lane & 1;  // odd lanes take the second token
+  const int odd = lane & 1;  // odd lanes take the second token
   const float got = __shfl_xor_sync(0xffffffffu, odd ? y0 : y1, 1);
-  if (in && (!odd || second)) {
+  if (in && odd < left) {
     OutT* dst = static_cast<OutT*>(g.out) + (m + odd) * g.ldo + (col & ~1);
     *reinterpret_cast<uint32_t*>(dst) = odd ? pack2<OutT>(got, y1) : pack2<OutT>(y0, got);
   }
@@ -197,10 +198,9 @@ __device__ __forceinline__ void store_tile(const Fp4Args& g, const RowConsts& c,
     tmem_ld_wait();
 #pragma unroll
     for (int j = 0; j < 8; j += 2)
-      if (t + j < tokens)  // the same for the whole warp
-        store_tokens<EPI, OutT>(g, c, m0 + t + j, t + j + 1 < tokens,
-                                *reinterpret_cast<const float2*>(sa + t + j),
-                                __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+      store_tokens<EPI, OutT>(g, c, m0 + t + j, tokens - t - j,
+                              *reinterpret_cast<const float2*>(sa + t + j), __uint_as_float(r[j]),
+                              __uint_as_float(r[j + 1]));
   }
 }
 
@@ -249,7 +249,7 @@ __device__ __forceinline__ void store_reduced(const Fp4Args& g, const RowConsts&
       a0 += part[s].x;
       a1 += part[s].y;
     }
-    store_tokens<EPI, OutT>(g, c, m0 + 2 * p, 2 * p + 1 < tokens,
+    store_tokens<EPI, OutT>(g, c, m0 + 2 * p, tokens - 2 * p,
                             *reinterpret_cast<const float2*>(sa + 2 * p), a0, a1);
   }
 }
@@ -1002,16 +1002,17 @@ struct Fp4Choice {
 };
 
 // Measured on a B200 (back to back, us): one wave of 128 x 128 tiles is ahead of
-// the pair kernel (512 x 3072 x 3072: 8.2 against 10.1; 1003 x 1160 x 1376: 7.6
-// against 9.5), two waves are behind it (1024 x 3072 x 3072: 11.0 against 10.5;
-// 512 x 12288 x 3072: 20.2 against 16.0), so more than 128 tokens take the small
-// kernel only while its tiles fit the SMs at once.  Up to 128 tokens the weight is
-// read once either way, by twice the CTAs (128 x 12288 x 3072: 9.2 against 10.5).
+// the pair kernel (512 x 3072 x 3072: 7.6 against 10.3; 1003 x 1160 x 1376: 6.9
+// against 9.8), two waves are level or behind (1024 x 3072 x 3072: 10.3 against
+// 10.7; 256 x 12288 x 3072: 11.5 against 10.9; 512 x 12288 x 3072: 18.9 against
+// 16.6), so more than 128 tokens take the small kernel only while its tiles fit the
+// SMs at once.  Up to 128 tokens the weight is read once either way, by twice the
+// CTAs (128 x 12288 x 3072: 8.5 against 10.8).
 //
 // Slices of K: about 0.2 us a k-block, against 0.7 us and what grows with the
 // slices and tokens for the partial sums; only while every slice has an SM of its
-// own (1 x 3072 x 12288: 12.4, 7.6, 6.2 us with 1, 2, 4 slices; 48 x 3072 x 12288
-// mxfp4: 12.7, 9.1, 7.2; 256 x 3072 x 3072: 7.8, 8.9, 13.8).
+// own (1 x 3072 x 12288: 12.3, 7.5, 6.2 us with 1, 2, 4 slices; 48 x 3072 x 12288
+// mxfp4: 12.5, 8.8, 6.9; 256 x 3072 x 3072: 7.1, 8.8, 13.7).
 Fp4Choice pick_fp4(int64_t m, int64_t n, int kblocks, const Fp4Device& dev) {
   Fp4Choice c{m <= 32 ? 32 : m <= 64 ? 64 : 128, 1};
   const int64_t tiles = (m + c.tile - 1) / c.tile * ((n + kTileRows - 1) / kTileRows);
