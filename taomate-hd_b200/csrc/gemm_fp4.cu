@@ -1060,7 +1060,7 @@ int scaled_mm_fp4_impl(void* out, int out_dtype, const uint8_t* a, const uint8_t
   if (ldo < ((epilogue & TM_EPI_SWIGLU) ? n / 2 : n)) return TM_ERR_SHAPE;
   if (out_dtype != TM_DTYPE_BF16 && out_dtype != TM_DTYPE_FP16) return TM_ERR_DTYPE;
   if (m == 0) return TM_OK;
-  if (m > 0x7fffffffLL - 256 || n > 0x7fffffffLL - 256 || k > 0x7fffffffLL) return TM_ERR_TOO_LARGE;
+  if (m > 0x7fffffffLL - 256 || n > 0x7fffffffLL - 256 || k > (1ll << 30)) return TM_ERR_TOO_LARGE;
   if (!out || !a || !b || !blocks_a || !blocks_b) return TM_ERR_NULL_POINTER;
   if (sa && sa_numel != 1 && sa_numel != m) return TM_ERR_SHAPE;
   if (sb && sb_numel != 1 && sb_numel != n) return TM_ERR_SHAPE;

@@ -17,6 +17,8 @@ the same linears inside its DiT block, model/layers.py:346-368, :502-523):
                        out-projection with an all-reduce (NCCL, or fused into
                        the GEMM launch over NVLink peer memory).
 * ``TPW8A8BlockChain`` QKV, out-proj, fc1, fc2 of one block in sequence.
+* ``TPW4A4MLP``        the MLP of ``TPW8A8MLP`` with 4-bit weights and activations
+                       (nvfp4 or mxfp4 blocks), its partials reduced by NCCL.
 
 Every ``forward`` writes into buffers allocated at construction, so a step
 allocates nothing and can be captured in a CUDA graph.  Weights are random
@@ -193,6 +195,81 @@ class TPW8A8MLP:
         _gemm(self.q2, self.fc2, self.partial, bias=bias2)
         if gemm_events is not None:
             gemm_events[3].record()
+        t = self.ctx.tp_world_size
+        if t == 1:
+            return self.partial
+        if self.reduce == "reduce_scatter":
+            return reduce_scatter_rows(self.partial, group=self.ctx.tp_group, world_size=t,
+                                       out=self.out)
+        return all_reduce_sum_inplace_(self.partial, group=self.ctx.tp_group, world_size=t)
+
+
+@dataclass
+class W4Weight:
+    """4-bit weight of a linear [N, K]: codes [N, K / 2], block scales, fp32
+    row scales (nvfp4) and optional bias [N]."""
+
+    q: torch.Tensor
+    blocks: torch.Tensor
+    scale: torch.Tensor | None
+    bias: torch.Tensor | None
+
+
+class _Fp4Quant:
+    """Preallocated 4-bit activation buffers."""
+
+    def __init__(self, rows: int, cols: int, device: torch.device, block_format: str):
+        x = torch.empty(rows, cols, dtype=torch.bfloat16, device=device)
+        self.q, self.blocks, self.s = ops.scaled_fp4_quant(x.zero_(), block_format=block_format)
+
+    def __call__(self, x: torch.Tensor) -> None:
+        torch.ops.taomate_w8a8.scaled_fp4_quant(self.q, self.blocks, self.s, x, None)
+
+
+def _gemm_fp4(q: _Fp4Quant, w: W4Weight, out: torch.Tensor, *, bias: torch.Tensor | None,
+              gelu: bool = False) -> torch.Tensor:
+    torch.ops.taomate_w8a8.scaled_mm_fp4(out, q.q, w.q.t(), q.blocks, w.blocks, q.s, w.scale, bias,
+                                         ops.EPI_GELU_TANH if gelu else 0, 0, 1)
+    return out
+
+
+class TPW4A4MLP:
+    """The MLP of :class:`TPW8A8MLP` at 4 bits: fc1 column-parallel (+bias,
+    GELU-tanh in the epilogue) -> quant over the local K -> fc2 row-parallel,
+    partials summed by NCCL.  The same random weights, quantised after
+    sharding; TP rank 0 adds fc2's bias in its epilogue."""
+
+    def __init__(self, tokens: int, d: int, ffn: int, ctx: ParallelContext, device: torch.device,
+                 *, seed: int = 0, block_format: str = "nvfp4", reduce: str = "reduce_scatter"):
+        t, r = ctx.tp_world_size, ctx.tp_rank
+        if ffn % t or (ffn // t) % 32 or d % 32:
+            raise ValueError("d and the local ffn must be multiples of 32")
+        if reduce not in ("reduce_scatter", "all_reduce"):
+            raise ValueError("reduce must be 'reduce_scatter' or 'all_reduce'")
+        if reduce == "reduce_scatter" and tokens % t:
+            raise ValueError("tokens must divide by the TP degree")
+        self.ctx, self.tokens, self.d, self.ffn, self.reduce = ctx, tokens, d, ffn, reduce
+        w1 = column_slice(random_bf16((ffn, d), 0.02, seed + 10, device), t, r)
+        w2 = row_slice(random_bf16((d, ffn), 0.02, seed + 20, device), t, r)
+        b1 = column_slice(random_bf16((ffn,), 0.01, seed + 11, device), t, r)
+        b2 = random_bf16((d,), 0.01, seed + 21, device)
+        self.fc1 = W4Weight(*ops.scaled_fp4_quant(w1, block_format=block_format), b1)
+        self.fc2 = W4Weight(*ops.scaled_fp4_quant(w2, block_format=block_format), b2)
+        self.q1 = _Fp4Quant(tokens, d, device, block_format)
+        self.h = torch.empty(tokens, ffn // t, dtype=torch.bfloat16, device=device)
+        self.q2 = _Fp4Quant(tokens, ffn // t, device, block_format)
+        self.partial = torch.empty(tokens, d, dtype=torch.bfloat16, device=device)
+        self.out = torch.empty(tokens // t if reduce == "reduce_scatter" else tokens, d,
+                               dtype=torch.bfloat16, device=device)
+
+    launches_per_step = 4  # 2 quant + 2 GEMM
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        self.q1(x)
+        _gemm_fp4(self.q1, self.fc1, self.h, bias=self.fc1.bias, gelu=True)
+        self.q2(self.h)
+        _gemm_fp4(self.q2, self.fc2, self.partial,
+                  bias=self.fc2.bias if self.ctx.tp_rank == 0 else None)
         t = self.ctx.tp_world_size
         if t == 1:
             return self.partial

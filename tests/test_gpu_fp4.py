@@ -299,3 +299,289 @@ def test_mm_pair_tile(tm_ops, cuda, m, n, k, act, dtype, fmt):
     _check_mm(out, *ops, bias, fmt, act)
     plain = tm_ops.scaled_mm_fp4(aq, wq.t(), ab, wb, asc, wsc, dtype, tile=1256)
     _check_mm(plain, *ops, None, fmt)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m", [1, 2, 33, 64, 65, 128, 129, 700])
+def test_mm_every_route(tm_ops, cuda, m, fmt):
+    """The chosen kernel at the token counts where the choice changes, long K."""
+    *ops, bias = _operands(tm_ops, cuda, m, 520, 5376, fmt, torch.bfloat16, m)
+    aq, ab, asc, wq, wb, wsc = ops
+    _check_mm(tm_ops.scaled_mm_fp4(aq, wq.t(), ab, wb, asc, wsc, bias=bias), *ops, bias, fmt)
+
+
+def _slots(n, offset, dtype, cuda, fill=0.0):
+    """n values that start `offset` elements into their storage."""
+    return torch.full((n + offset,), fill, dtype=dtype, device=cuda)[offset:]
+
+
+@pytest.mark.parametrize("tile", [0, 64, 1256])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_mm_strides_and_alignment(tm_ops, cuda, fmt, tile):
+    """Row-strided codes and output, scales and bias at odd addresses; what lies
+    beside the output stays as it was."""
+    m, n, k = 60, 392, 672
+    *ops, bias = _operands(tm_ops, cuda, m, n, k, fmt, torch.bfloat16, 5)
+    aq, ab, asc, wq, wb, wsc = ops
+    a_big = torch.randint(0, 255, (m, k // 2 + 48), dtype=torch.uint8, device=cuda)
+    w_big = torch.randint(0, 255, (n, k // 2 + 16), dtype=torch.uint8, device=cuda)
+    a_big[:, 16:16 + k // 2] = aq
+    w_big[:, :k // 2] = wq
+    if wsc is not None:
+        asc, wsc = _slots(m, 1, torch.float32, cuda).copy_(asc.view(-1)), \
+            _slots(n, 3, torch.float32, cuda).copy_(wsc.view(-1))
+    bias = _slots(n, 1, torch.bfloat16, cuda).copy_(bias)
+    for width, start in ((n + 8, 8), (n + 24, 16)):  # rows on 16- and on 32-byte boundaries
+        big = torch.full((m + 2, width), 7.0, dtype=torch.bfloat16, device=cuda)
+        out = big[1:m + 1, start:start + n]
+        if out.data_ptr() % 16:
+            continue
+        torch.ops.taomate_w8a8.scaled_mm_fp4(
+            out, a_big[:, 16:16 + k // 2], w_big[:, :k // 2].t(), ab, wb, asc, wsc, bias, 0, tile, 1)
+        _check_mm(out, aq, ab, asc, wq, wb, wsc, bias, fmt)
+        keep = torch.ones_like(big, dtype=torch.bool)
+        keep[1:m + 1, start:start + n] = False
+        assert (big[keep] == 7.0).all()
+
+
+@pytest.mark.parametrize("tile,splits", [(32, 1), (32, 4), (128, 2), (1256, 1)])
+def test_mm_scalar_scales_and_shapes(tm_ops, cuda, tile, splits):
+    """Per-tensor scales on either side, a given activation scale, 3-D input, `out`."""
+    m, n, k = 24, 136, 1024
+    x = orc.activation(m, k, 1, outlier_channels=None).bfloat16().to(cuda)
+    w = orc.weight(n, k, seed=2).to(cuda)
+    sx, sw = torch.tensor([0.002], device=cuda), torch.tensor([0.0001], device=cuda)
+    aq, ab, asc = tm_ops.scaled_fp4_quant(x, sx)
+    wq, wb, wsc = tm_ops.scaled_fp4_quant(w, sw)
+    out = torch.empty(m, n, dtype=torch.float16, device=cuda)
+    got = tm_ops.scaled_mm_fp4(aq, wq.t(), ab, wb, asc, wsc, out=out, tile=tile, splits=splits)
+    assert got is out
+    _check_mm(out, aq, ab, asc, wq, wb, wsc, None, "nvfp4")
+    q3, b3, s3 = tm_ops.scaled_fp4_quant(x.view(2, 12, k))
+    assert q3.shape == (2, 12, k // 2) and s3.shape == (m, 1)
+    y3 = tm_ops.scaled_mm_fp4(q3, wq.t(), b3, wb, s3, wsc)
+    assert y3.shape == (2, 12, n)
+    _check_mm(y3.view(m, n), q3.view(m, -1), b3, s3, wq, wb, wsc, None, "nvfp4")
+    assert tm_ops.scaled_mm_fp4(aq[:0], wq.t(), *tm_ops.scaled_fp4_quant(x[:0])[1:2], wb,
+                                asc, wsc).shape == (0, n)
+
+
+@pytest.mark.parametrize("tile", [32, 1256])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_mm_nan_rows(tm_ops, cuda, fmt, tile):
+    """An inf or NaN in a token makes its outputs NaN, in a weight row its
+    column's, and nothing else."""
+    x = orc.activation(20, 512, 1, outlier_channels=None).bfloat16()
+    w = orc.weight(72, 512, seed=2).clone()
+    x[3, 100], x[17, 511], w[40, 7] = float("nan"), float("inf"), float("-inf")
+    x[5] = 0.0
+    a, b = (tm_ops.scaled_fp4_quant(t.to(cuda), block_format=fmt) for t in (x, w))
+    y = tm_ops.scaled_mm_fp4(a[0], b[0].t(), a[1], b[1], a[2], b[2], tile=tile).cpu()
+    bad = torch.zeros(20, 72, dtype=torch.bool)
+    bad[3], bad[17], bad[:, 40] = True, True, True
+    assert torch.equal(torch.isnan(y), bad)
+    assert (y[5][~bad[5]] == 0).all()
+
+
+def test_streams_and_graphs(tm_ops, cuda):
+    """Two streams at once, and two captured graphs replayed on new inputs while
+    eager calls run: the calls share no scratch memory."""
+    shapes = [(1, 1024, 4096), (48, 640, 5376), (300, 1344, 800), (2100, 4160, 544)]
+    cases = []
+    for m, n, k in shapes:
+        x = orc.activation(m, k, m, outlier_channels=None).bfloat16().to(cuda)
+        w = tm_ops.scaled_fp4_quant(orc.weight(n, k, seed=n).to(cuda))
+        cases.append((x, w))
+
+    def linear(x, w):
+        q, b, s = tm_ops.scaled_fp4_quant(x)
+        return tm_ops.scaled_mm_fp4(q, w[0].t(), b, w[1], s, w[2], gelu_tanh=True)
+
+    want = [linear(x, w) for x, w in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = [linear(x, w) for x, w in (cases if i else cases[::-1])]
+    torch.cuda.synchronize()
+    for a, b, c in zip(want, got[1], got[0][::-1]):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+    graphs, outs = [], []
+    inputs = [x.clone() for x, _ in cases]
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append([linear(x, w) for x, (_, w) in zip(inputs, cases)])
+        graphs.append(g)
+    for x in inputs:
+        x.mul_(0.5).neg_()
+    torch.cuda.synchronize()
+    for i, g in enumerate(graphs):
+        with torch.cuda.stream(streams[i]):
+            g.replay()
+    eager = [linear(x, w) for x, (_, w) in zip(inputs, cases)]
+    torch.cuda.synchronize()
+    for g in graphs:
+        g.replay()
+    torch.cuda.synchronize()
+    for o in outs:
+        for a, b in zip(o, eager):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_positions_past_32_bits(tm_ops, cuda, fmt):
+    """More than 2^31 elements on either side of the quantisation, and an output of
+    more than 2^31 elements: the far rows equal those of small calls."""
+    rows, cols = 70_000, 32_768  # 2.3e9 elements
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device=cuda)
+    tail = orc.activation(130, cols, 3, outlier_channels=None).bfloat16().to(cuda)
+    x[-130:] = tail
+    q, b, s = tm_ops.scaled_fp4_quant(x, block_format=fmt)
+    qt, _, st = tm_ops.scaled_fp4_quant(tail, block_format=fmt)
+    assert torch.equal(q[-130:], qt) and (s is None or torch.equal(s[-130:], st))
+    y = tm_ops.dequantize_fp4(q, b, s)
+    assert torch.equal(y[-130:], tm_ops.dequantize_fp4(*tm_ops.scaled_fp4_quant(tail, block_format=fmt)))
+    assert not y[:1000].any()
+    del x, y
+    w = tm_ops.scaled_fp4_quant(orc.weight(34_000, 64, seed=1).to(cuda), block_format=fmt)
+    a = tm_ops.scaled_fp4_quant(orc.activation(rows, 64, 2, outlier_channels=None).bfloat16().to(cuda),
+                                block_format=fmt)
+    out = tm_ops.scaled_mm_fp4(a[0], w[0].t(), a[1], w[1], a[2], w[2])  # 2.4e9 outputs
+    last = a[0][-100:].contiguous()
+    va = _values(*a, fmt)[-100:]
+    ref = va @ _values(*w, fmt).T
+    size = np.abs(va) @ np.abs(_values(*w, fmt)).T
+    err = np.abs(out[-100:].cpu().double().numpy() - ref)
+    assert last.shape == (100, 32)
+    assert (err <= 2.0 ** -8 * np.abs(ref) + (64 / 16 + 16) * 2.0 ** -22 * size).all()
+
+
+def test_c_abi_linear(tm_ops, capi, cuda):
+    """Quantisation, product and inverse through the C ABI alone."""
+    m, n, k = 70, 200, 416
+    x = orc.activation(m, k, 1, outlier_channels=None).bfloat16().to(cuda)
+    w = orc.weight(n, k, seed=2).to(cuda)
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    for code, fmt in ((0, "nvfp4"), (1, "mxfp4")):
+        parts = []
+        for t, rows, dt in ((x, m, 0), (w, n, {torch.bfloat16: 0, torch.float32: 2}[w.dtype])):
+            size = ctypes.c_uint64()
+            assert capi.tm_fp4_block_scales_size(rows, k, code, ctypes.byref(size)) == 0
+            q = torch.empty(rows, k // 2, dtype=torch.uint8, device=cuda)
+            blocks = torch.empty(size.value, dtype=torch.uint8, device=cuda)
+            s = torch.empty(rows, device=cuda) if code == 0 else None
+            assert capi.tm_scaled_fp4_quant(q.data_ptr(), blocks.data_ptr(),
+                                            None if s is None else s.data_ptr(), None, t.data_ptr(),
+                                            dt, code, rows, k, k, stream) == 0
+            ref = tm_ops.scaled_fp4_quant(t, block_format=fmt)
+            assert torch.equal(q, ref[0]) and torch.equal(blocks, ref[1].view(torch.uint8).view(-1))
+            back = torch.empty(rows, k, dtype=torch.float32, device=cuda)
+            assert capi.tm_dequantize_fp4(back.data_ptr(), 2, q.data_ptr(), blocks.data_ptr(),
+                                          None if s is None else s.data_ptr(), rows if s is not None else 0,
+                                          code, rows, k, stream) == 0
+            assert torch.equal(back, tm_ops.dequantize_fp4(*ref, torch.float32))
+            parts.append((q, blocks, s))
+        (aq, ab, sa), (wq, wb, sw) = parts
+        out = torch.empty(m, n, dtype=torch.bfloat16, device=cuda)
+        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        assert capi.tm_scaled_mm_fp4(ptr(out), 0, ptr(aq), ptr(wq), ptr(ab), ptr(wb), ptr(sa),
+                                     m if sa is not None else 0, ptr(sw), n if sw is not None else 0,
+                                     None, code, m, n, k, k // 2, k // 2, n, 0, stream) == 0
+        kind = torch.float8_e4m3fn if code == 0 else torch.float8_e8m0fnu
+        shape = f4.scale_tiles(m, k, fmt), f4.scale_tiles(n, k, fmt)
+        _check_mm(out, aq, ab.view(shape[0]).view(kind), sa, wq, wb.view(shape[1]).view(kind), sw,
+                  None, fmt)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_block_run(tm_ops, cuda, fmt):
+    """A block's MLP as it is used: gated residual + RMSNorm + modulate producer,
+    fc1 with bias and GELU, quantisation, fc2.  Each product is held to the
+    64-bit value of its own stored operands, each quantisation to every bit."""
+    tokens, d, ffn = 333, 512, 1408
+    g = torch.Generator().manual_seed(4)
+    rnd = lambda *shape, std=1.0: (torch.randn(shape, generator=g) * std).bfloat16().to(cuda)  # noqa: E731
+    residual, branch, weight = rnd(tokens, d), rnd(tokens, d), 1 + rnd(d, std=0.1)
+    shift, scale, gate = (rnd(3, d, std=0.3) for _ in range(3))
+    index = torch.randint(0, 3, (tokens,), generator=g).to(cuda)
+    w1 = tm_ops.scaled_fp4_quant(rnd(ffn, d, std=0.05), block_format=fmt)
+    w2 = tm_ops.scaled_fp4_quant(rnd(d, ffn, std=0.05), block_format=fmt)
+    b1, b2 = rnd(ffn, std=0.2), rnd(d, std=0.2)
+    q, b, s, new_residual, hidden = tm_ops.residual_gate_rms_norm_modulate_fp4_quant(
+        residual, branch, gate, weight, 1e-6, shift, scale, index, block_format=fmt,
+        return_hidden=True)
+    _check_quant((q, b, s), hidden.cpu(), fmt)
+    h = tm_ops.scaled_mm_fp4(q, w1[0].t(), b, w1[1], s, w1[2], bias=b1, gelu_tanh=True)
+    _check_mm(h, q, b, s, *w1, b1, fmt, "gelu")
+    q2, bb2, s2 = tm_ops.scaled_fp4_quant(h, block_format=fmt)
+    _check_quant((q2, bb2, s2), h.cpu(), fmt)
+    y = tm_ops.scaled_mm_fp4(q2, w2[0].t(), bb2, w2[1], s2, w2[2], bias=b2)
+    _check_mm(y, q2, bb2, s2, *w2, b2, fmt)
+    assert torch.isfinite(y).all() and new_residual.shape == residual.shape
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_dit_mlp_stage(tm_ops, cuda, fmt):
+    """dit.TPW4A4MLP is the operators in sequence, and can be captured."""
+    from taomate_hd_b200.dit import TPW4A4MLP
+    from taomate_hd_b200.parallel import ParallelContext
+
+    ctx = ParallelContext(tp_world_size=1, tp_rank=0, tp_group=None)
+    mlp = TPW4A4MLP(320, 256, 1024, ctx, cuda, seed=3, block_format=fmt)
+    x = orc.activation(320, 256, 7, outlier_channels=1).bfloat16().to(cuda)
+    got = mlp.forward(x).clone()
+    q, b, s = tm_ops.scaled_fp4_quant(x, block_format=fmt)
+    h = tm_ops.scaled_mm_fp4(q, mlp.fc1.q.t(), b, mlp.fc1.blocks, s, mlp.fc1.scale,
+                             bias=mlp.fc1.bias, gelu_tanh=True)
+    q, b, s = tm_ops.scaled_fp4_quant(h, block_format=fmt)
+    want = tm_ops.scaled_mm_fp4(q, mlp.fc2.q.t(), b, mlp.fc2.blocks, s, mlp.fc2.scale,
+                                bias=mlp.fc2.bias)
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = mlp.forward(x)
+    x.mul_(2.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, mlp.forward(x)) and not torch.equal(out, got)
+
+
+def test_refusals_on_device_tensors(tm_ops, cuda):
+    """Wrong types, shapes and formats raise before any launch."""
+    x = torch.zeros(4, 64, dtype=torch.bfloat16, device=cuda)
+    q, b, s = tm_ops.scaled_fp4_quant(x)
+    qm, bm, _ = tm_ops.scaled_fp4_quant(x, block_format="mxfp4")
+    one = torch.ones(1, device=cuda)
+    mm = tm_ops.scaled_mm_fp4
+    w = torch.zeros(8, 64, dtype=torch.bfloat16, device=cuda)
+    wq, wb, ws = tm_ops.scaled_fp4_quant(w)
+    bad = [
+        (lambda: tm_ops.scaled_fp4_quant(x.to(torch.int32)), RuntimeError),
+        (lambda: tm_ops.scaled_fp4_quant(x[:, :48]), RuntimeError),
+        (lambda: tm_ops.scaled_fp4_quant(x, one, block_format="mxfp4"), RuntimeError),
+        (lambda: tm_ops.scaled_fp4_quant(x, torch.ones(4, device=cuda)), RuntimeError),
+        (lambda: tm_ops.scaled_fp4_quant(x, block_format="fp4"), ValueError),
+        (lambda: tm_ops.dequantize_fp4(q, b), RuntimeError),           # nvfp4 needs its scales
+        (lambda: tm_ops.dequantize_fp4(qm, bm, one), RuntimeError),    # mxfp4 takes none
+        (lambda: tm_ops.dequantize_fp4(q, b[:, :0], s), RuntimeError),
+        (lambda: tm_ops.dequantize_fp4(q, b.view(torch.uint8), s), RuntimeError),
+        (lambda: tm_ops.dequantize_fp4(q, b, s, torch.int8), RuntimeError),
+        (lambda: mm(q, wq.t(), b, wb, s), RuntimeError),
+        (lambda: mm(q, wq.t(), b, bm, s, ws), RuntimeError),           # two formats
+        (lambda: mm(q, wq, b, wb, s, ws), RuntimeError),               # weight not transposed
+        (lambda: mm(q, wq.t(), b, wb, s, ws, torch.float32), RuntimeError),
+        (lambda: mm(q, wq.t(), b, wb, s, ws, bias=torch.zeros(8, device=cuda)), RuntimeError),
+        (lambda: mm(q, wq.t(), b, wb, s, ws, swiglu=True), RuntimeError),  # N % 64
+        (lambda: mm(q, wq.t(), b, wb, s, ws, gelu_tanh=True, swiglu=True), ValueError),
+        (lambda: mm(q, wq.t(), b, wb, s, ws, tile=48), RuntimeError),
+        (lambda: mm(q, wq.t(), b, wb, s, ws, tile=32, splits=2), RuntimeError),  # one k-block
+        (lambda: mm(q, wq.t(), b, wb, s, ws, out=torch.empty(4, 4, device=cuda)), RuntimeError),
+        (lambda: tm_ops.modulate_fp4_quant(x.float(), x[:1], x[:1], None), RuntimeError),
+    ]
+    for call, error in bad:
+        with pytest.raises(error):
+            call()
