@@ -826,7 +826,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(free_leader);
+      if (lane == 0) mbar_arrive_cluster_relaxed(free_leader);
       const int col0 = nb * kPairRows + 128 * h;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {

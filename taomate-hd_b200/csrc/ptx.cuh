@@ -353,6 +353,15 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
                : "memory");
 }
 
+// The same without release semantics: for handing back something whose last use
+// was a completed read (TMEM columns after tcgen05.wait::ld), where there is no
+// write to publish.  The release form waits for the thread's earlier memory
+// operations, about 1 us with stores in flight.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
+               : "memory");
+}
+
 // 2-D tile load into this CTA's shared memory whose completion is counted
 // on an mbarrier of the pair's leader CTA (`bar_cluster` from map_to_cta).
 // Each CTA of the pair fetches its own half of the operands.
