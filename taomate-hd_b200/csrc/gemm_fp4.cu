@@ -588,10 +588,11 @@ __device__ __forceinline__ void pair_finish16(uint32_t* r, uint64_t sa2, bool ha
 }
 
 // Store 16 columns of this lane's row, as one 32-byte sector where the output
-// allows it (`wide`: rows start on 32-byte boundaries).  Straight from
-// registers: staged TMA stores would wait in the queue of the operand loads.
-// Two 16-byte stores in place of the one cost 8192 x 12288 x 3072 nvfp4
-// 197 against 150 us.
+// allows it (`wide`: rows start on 32-byte boundaries).  8192 x 12288 x 3072
+// nvfp4: two 16-byte stores in place of the one cost 197 against 150 us; staged
+// TMA stores, or full lines after an exchange between lanes, gain nothing (121
+// and 128 against 123 us): what remains is the output's share of the traffic.
+// Not allocating in L1: with GELU 134 -> 129 us.
 template <typename OutT>
 __device__ __forceinline__ void pair_store16(OutT* row, const uint32_t* y, int col, int cols,
                                              bool wide) {
@@ -601,7 +602,7 @@ __device__ __forceinline__ void pair_store16(OutT* row, const uint32_t* y, int c
     w[i] = pack2<OutT>(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]));
   OutT* dst = row + col;
   if (wide && col + 16 <= cols) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(w[0]),
+    asm volatile("st.global.L1::no_allocate.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(w[0]),
                  "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                  : "memory");
   } else {  // columns come in multiples of 8

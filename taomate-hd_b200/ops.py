@@ -215,7 +215,7 @@ def scaled_fp4_quant(
     call: their rows are the output channels.  A row (or block) that holds an
     infinity or a NaN becomes NaN as a whole.
     """
-    _require_cuda(input, scale)
+    _require_cuda(input)
     return _ops.scaled_fp4_quant_new.default(input, scale, _is_mx(block_format))
 
 
@@ -227,7 +227,7 @@ def dequantize_fp4(
 ) -> torch.Tensor:
     """The values of a tensor quantised by :func:`scaled_fp4_quant`, ``[..., K]``
     in ``out_dtype`` (bf16, fp16 or fp32): what a layer would see at 4 bits."""
-    _require_cuda(q, block_scales, scales)
+    _require_cuda(q)
     return _ops.dequantize_fp4_new.default(q, block_scales, scales, out_dtype)
 
 
@@ -259,7 +259,7 @@ def scaled_mm_fp4(
     activation.  ``out`` ([M, N] or [M, N / 2]) makes the call allocation-free;
     ``tile`` and ``splits`` force a kernel configuration (0 = heuristic).
     """
-    _require_cuda(a, b, block_scale_a, block_scale_b, scale_a, scale_b, bias, out)
+    _require_cuda(a)  # the operator checks that the others are on its device
     if gelu_tanh and swiglu:
         raise ValueError("gelu_tanh and swiglu are exclusive")
     epi = (EPI_GELU_TANH if gelu_tanh else 0) | (EPI_SWIGLU if swiglu else 0)
@@ -439,7 +439,7 @@ def modulate_fp4_quant(
     """:func:`modulate_int8_quant` with 4-bit output: returns ``(codes,
     block_scales, scales or None, hidden or None)``, the hidden state the same
     bits as the int8 producer's, quantised as by :func:`scaled_fp4_quant`."""
-    _require_cuda(x, shift, scale, index)
+    _require_cuda(x)
     return _ops.modulate_fp4_quant_new.default(x, shift, scale, index, _is_mx(block_format),
                                                return_hidden)
 
@@ -457,7 +457,7 @@ def rms_norm_modulate_fp4_quant(
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
     """:func:`rms_norm_modulate_int8_quant` with 4-bit output
     (:func:`modulate_fp4_quant`)."""
-    _require_cuda(x, weight, shift, scale, index)
+    _require_cuda(x)
     return _ops.rms_norm_modulate_fp4_quant_new.default(
         x, weight, float(eps), shift, scale, index, _is_mx(block_format), return_hidden)
 
@@ -478,7 +478,7 @@ def residual_gate_rms_norm_modulate_fp4_quant(
     """:func:`residual_gate_rms_norm_modulate_int8_quant` with 4-bit output:
     returns ``(codes, block_scales, scales or None, updated residual, hidden
     or None)``."""
-    _require_cuda(residual, branch, gate, weight, shift, scale, index)
+    _require_cuda(residual)
     return _ops.residual_gate_rms_norm_modulate_fp4_quant_new.default(
         residual, branch, gate, weight, float(eps), shift, scale, index, _is_mx(block_format),
         return_hidden)
