@@ -9,7 +9,7 @@
 // cutlass_scaled_mm / scaled_mm_i8_ex (cached per device and stream, from
 // torch's caching allocator) for shapes that use split-K.
 #include <ATen/cuda/CUDAContext.h>
-#include <ATen/ops/empty.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty_like.h>
 #include <ATen/ops/zeros.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -729,6 +729,12 @@ void scaled_mm_fp4(at::Tensor& out, const at::Tensor& a, const at::Tensor& b,
 }
 
 // ---- the allocating forms, one dispatcher call each (the Python API) ----
+// Contiguous and uninitialised, from the caching allocator without another
+// pass through the dispatcher.
+at::Tensor empty_on(const at::Tensor& like, at::IntArrayRef sizes, at::ScalarType dtype) {
+  return at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt);
+}
+
 struct Fp4Tensors {
   at::Tensor q, blocks;
   std::optional<at::Tensor> scales;
@@ -743,11 +749,11 @@ Fp4Tensors empty_fp4(const at::Tensor& like, bool mx, bool row_scales) {
   Fp4Tensors t;
   at::DimVector sizes(like.sizes());
   sizes.back() = cols / 2;
-  t.q = at::empty(sizes, like.options().dtype(at::kByte));
+  t.q = empty_on(like, sizes, at::kByte);
   const int64_t blocks = cols / (mx ? 32 : 16);
-  t.blocks = at::empty({(rows + 127) / 128 * 128, (blocks + 3) / 4 * 4},
-                       like.options().dtype(mx ? at::kFloat8_e8m0fnu : at::kFloat8_e4m3fn));
-  if (row_scales && !mx) t.scales = at::empty({rows, 1}, like.options().dtype(at::kFloat));
+  t.blocks = empty_on(like, {(rows + 127) / 128 * 128, (blocks + 3) / 4 * 4},
+                      mx ? at::kFloat8_e8m0fnu : at::kFloat8_e4m3fn);
+  if (row_scales && !mx) t.scales = empty_on(like, {rows, 1}, at::kFloat);
   return t;
 }
 
@@ -769,7 +775,7 @@ at::Tensor dequantize_fp4_new(const at::Tensor& q, const at::Tensor& block_scale
   const c10::cuda::CUDAGuard guard(q.device());
   at::DimVector sizes(q.sizes());
   sizes.back() *= 2;
-  at::Tensor out = at::empty(sizes, q.options().dtype(dtype));
+  at::Tensor out = empty_on(q, sizes, dtype);
   dequantize_fp4(out, q.contiguous(), block_scales, scales);
   return out;
 }
@@ -784,7 +790,7 @@ at::Tensor scaled_mm_fp4_new(const at::Tensor& a, const at::Tensor& b,
   const c10::cuda::CUDAGuard guard(a.device());
   const at::Tensor a2 = a.dim() == 2 ? a : a.reshape({a.numel() / a.size(-1), a.size(-1)});
   const int64_t cols = (epilogue & TM_EPI_SWIGLU) ? b.size(1) / 2 : b.size(1);
-  at::Tensor out = at::empty({a2.size(0), cols}, a.options().dtype(dtype));
+  at::Tensor out = empty_on(a, {a2.size(0), cols}, dtype);
   scaled_mm_fp4(out, a2, b, block_scales_a, block_scales_b, scales_a, scales_b, bias, epilogue, 0,
                 1);
   if (a.dim() == 2) return out;
