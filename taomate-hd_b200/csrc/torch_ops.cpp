@@ -764,7 +764,9 @@ Fp4Result scaled_fp4_quant_new(const at::Tensor& input, const std::optional<at::
   TORCH_CHECK(!mx || !scale.has_value(), "blocks of 32 take no fp32 scale");
   const c10::cuda::CUDAGuard guard(input.device());
   Fp4Tensors t = empty_fp4(input, mx, !scale.has_value());
-  const bool rows = input.dim() == 2 && input.stride(1) == 1;
+  // rows may be any distance apart, but not overlap (an expanded or windowed view)
+  const bool rows = input.dim() == 2 && input.stride(1) == 1 &&
+                    (input.size(0) <= 1 || input.stride(0) >= input.size(1));
   scaled_fp4_quant(t.q, t.blocks, t.scales, rows ? input : input.contiguous(), scale);
   return {t.q, t.blocks, scale.has_value() ? scale : t.scales};
 }

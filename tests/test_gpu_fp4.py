@@ -59,7 +59,7 @@ def _borders(dtype):
     rows = []
     for mantissa in range(8):
         s = 1.0 + mantissa / 8
-        for top in (6.0, 5.0, 4.5):
+        for top in (6.0, 5.0, 4.5, 5.25):  # 5.25 = 21 / 4: a row scale that is exact
             t = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], dtype=torch.float64)
             step = torch.finfo(dtype).eps
             near = torch.cat((t, t * (1 + step), t * (1 - step)))
@@ -117,11 +117,35 @@ def test_quant_extreme_rows(tm_ops, cuda, dtype, fmt):
                      0.01)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_quant_ties_under_every_row_maximum(tm_ops, cuda, dtype):
+    """Every significand of a row maximum a (p bits), against elements that make
+    x / (a / 2688 s) a border exactly, or miss one by a unit in the last place."""
+    p = 8 if dtype == torch.bfloat16 else 11
+    a = torch.arange(1 << (p - 1), 1 << p, dtype=torch.float64)
+    if len(a) > 300:
+        a = a[:: 7]
+    t = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], dtype=torch.float64)
+    s = torch.arange(8, 16, dtype=torch.float64)
+    want = a.view(-1, 1, 1) / 2688 * s.view(1, -1, 1) * 16 * t.view(1, 1, -1)  # [a, s, t]
+    x = torch.zeros(len(a), 8, 32, dtype=torch.float64)
+    step = torch.finfo(dtype).eps
+    x[:, :, 0:7], x[:, :, 7:14] = want, -want * (1 + step)
+    x[:, :, 16:23], x[:, :, 23:30] = want * (1 - step), want
+    # the element that gives the block its scale s: 6 s of the unit
+    x[:, :, 14] = x[:, :, 30] = a.view(-1, 1) / 2688 * s * 16 * 6
+    x = torch.cat((x.reshape(len(a), -1), torch.zeros(len(a), 32, dtype=torch.float64)), 1)
+    x[:, -1] = a  # the row maximum
+    x = x.to(dtype)
+    _check_quant(tm_ops.scaled_fp4_quant(x.to(cuda)), x, "nvfp4")
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_quant_strides_and_alignment(tm_ops, cuda, fmt):
     big = orc.activation(40, 1024, 6, outlier_channels=None).bfloat16().to(cuda)
     for view in (big[:, :512], big[:, 8:520], big[:, 16:528], big[3:, 1:129], big[::2, :96],
-                 big.reshape(8, 5, 1024), big.t()[:, :32], big[:, ::2]):
+                 big.reshape(8, 5, 1024), big.t()[:, :32], big[:, ::2], big[:1, :64].expand(9, 64),
+                 big.view(-1).as_strided((30, 64), (32, 1)), big[0, :96]):
         _check_quant(tm_ops.scaled_fp4_quant(view, block_format=fmt), view.cpu().contiguous(), fmt)
     f = big.float()
     for view in (f[:, 4:516], f[:, 1:65]):
