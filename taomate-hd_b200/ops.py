@@ -18,6 +18,10 @@ from ._native import load_torch_ops
 
 load_torch_ops()
 _ops = torch.ops.taomate_w8a8
+# the allocating 4-bit operators, looked up once (the smallest calls are bound by CPU time)
+_scaled_fp4_quant = _ops.scaled_fp4_quant_new.default
+_dequantize_fp4 = _ops.dequantize_fp4_new.default
+_scaled_mm_fp4 = _ops.scaled_mm_fp4_new.default
 
 EPI_GELU_TANH = 0x1
 EPI_SWIGLU = 0x2
@@ -216,7 +220,7 @@ def scaled_fp4_quant(
     infinity or a NaN becomes NaN as a whole.
     """
     _require_cuda(input)
-    return _ops.scaled_fp4_quant_new.default(input, scale, _is_mx(block_format))
+    return _scaled_fp4_quant(input, scale, _is_mx(block_format))
 
 
 def dequantize_fp4(
@@ -228,7 +232,7 @@ def dequantize_fp4(
     """The values of a tensor quantised by :func:`scaled_fp4_quant`, ``[..., K]``
     in ``out_dtype`` (bf16, fp16 or fp32): what a layer would see at 4 bits."""
     _require_cuda(q)
-    return _ops.dequantize_fp4_new.default(q, block_scales, scales, out_dtype)
+    return _dequantize_fp4(q, block_scales, scales, out_dtype)
 
 
 def scaled_mm_fp4(
@@ -264,8 +268,8 @@ def scaled_mm_fp4(
         raise ValueError("gelu_tanh and swiglu are exclusive")
     epi = (EPI_GELU_TANH if gelu_tanh else 0) | (EPI_SWIGLU if swiglu else 0)
     if out is None and tile == 0:
-        return _ops.scaled_mm_fp4_new.default(a, b, block_scale_a, block_scale_b, scale_a, scale_b,
-                                              out_dtype, bias, epi)
+        return _scaled_mm_fp4(a, b, block_scale_a, block_scale_b, scale_a, scale_b, out_dtype, bias,
+                              epi)
     a2 = a.reshape(-1, a.shape[-1])
     if out is None:
         cols = b.shape[1] // 2 if swiglu else b.shape[1]
