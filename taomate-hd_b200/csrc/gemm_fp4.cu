@@ -590,8 +590,9 @@ __device__ __forceinline__ void pair_finish16(uint32_t* r, uint64_t sa2, bool ha
 // Store 16 columns of this lane's row, as one 32-byte sector where the output
 // allows it (`wide`: rows start on 32-byte boundaries).  8192 x 12288 x 3072
 // nvfp4: two 16-byte stores in place of the one cost 197 against 150 us; staged
-// TMA stores, or full lines after an exchange between lanes, gain nothing (121
-// and 128 against 123 us): what remains is the output's share of the traffic.
+// TMA stores (121 against 123), or full lines after an exchange between lanes
+// (mxfp4 117 against 111), gain nothing: what remains is the output's share of
+// the traffic.
 // Not allocating in L1: with GELU 134 -> 129 us.
 template <typename OutT>
 __device__ __forceinline__ void pair_store16(OutT* row, const uint32_t* y, int col, int cols,
