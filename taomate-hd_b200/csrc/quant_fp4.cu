@@ -183,11 +183,11 @@ __device__ __forceinline__ uint32_t scaled_codes8(const float (&x)[8], float inv
 }
 
 // 32 bytes that no kernel in flight writes; `wide`: the address is a multiple of
-// 32 (one load), else of 16.  Not volatile: an unrolled loop's loads may all be
-// issued ahead of its stores.
+// 32 (one load), else of 16.  Volatile, so that it stays behind griddep_wait(); the
+// loads of an unrolled loop are still issued ahead of its stores (timed: no difference).
 __device__ __forceinline__ void ld_stream32(const void* p, bool wide, uint4& a, uint4& b) {
   if (wide) {
-    asm("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z),
                    "=r"(b.w)
                  : "l"(p));
@@ -195,6 +195,23 @@ __device__ __forceinline__ void ld_stream32(const void* p, bool wide, uint4& a, 
     a = ld_cached16(p);
     b = ld_cached16(static_cast<const uint8_t*>(p) + 16);
   }
+}
+
+// 32 bytes of a table row that other rows may share: kept in L1.
+__device__ __forceinline__ void ld_table32(const void* p, bool wide, uint4& a, uint4& b) {
+  if (wide) {
+    asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z),
+                   "=r"(b.w)
+                 : "l"(p));
+  } else {
+    a = ld_cached16(p);
+    b = ld_cached16(static_cast<const uint8_t*>(p) + 16);
+  }
+}
+
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
 }
 
 // 32 bytes to a multiple of 32.
@@ -462,6 +479,15 @@ __device__ __forceinline__ float row_rms_inverse(const Fp4Params& p, Unit<__nv_b
   return rsqrt_two_step_rn(__fadd_rn(variance, p.eps));
 }
 
+__host__ __device__ constexpr bool has_residual(int mode) {
+  return mode == kResGateRmsModulate || mode == kResGateRmsModulateRows;
+}
+
+// Producers with a norm whose rows have tables of their own.
+__host__ __device__ constexpr bool norm_rows(int mode) {
+  return mode == kRmsModulateRows || mode == kResGateRmsModulateRows;
+}
+
 // A producer applied to the row's units, in place; also writes the updated
 // residual and the hidden state where there are such outputs.
 template <int VPT, int MODE>
@@ -471,9 +497,10 @@ __device__ __forceinline__ void adaln_units(const Fp4Params& p, Unit<__nv_bfloat
   using U = Unit<__nv_bfloat16>;
   const int64_t trow = active ? (p.index ? p.index[row] : row) : 0;
   const auto unit_of = [&](int i) { return t + i * tpr; };
+  // 32-byte table loads in the producers without a norm: 41 -> 39 us (nvfp4) and 37 -> 34
+  // (mxfp4) at 20480 x 3072 with five tables; with a norm they change nothing (70, 66 us).
   const auto load = [&](U& v, const __nv_bfloat16* at, int unit) {
-    v.raw[0] = ld_cached16(at + unit * 16);
-    v.raw[1] = ld_cached16(at + unit * 16 + 8);
+    ld_table32(at + unit * 16, wide && modulate_only(MODE), v.raw[0], v.raw[1]);
   };
   const auto store = [&](__nv_bfloat16* at, int unit, const U& v) {
     uint4* dst = reinterpret_cast<uint4*>(at + (row * p.cols + unit * 16));
@@ -494,7 +521,7 @@ __device__ __forceinline__ void adaln_units(const Fp4Params& p, Unit<__nv_bfloat
         load(pre_sh[i], p.shift + trow * p.table_stride, unit_of(i));
       }
   }
-  if constexpr (MODE == kResGateRmsModulate) {
+  if constexpr (has_residual(MODE)) {
     const __nv_bfloat16* branch = p.branch + row * p.cols;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -509,6 +536,17 @@ __device__ __forceinline__ void adaln_units(const Fp4Params& p, Unit<__nv_bfloat
         store(p.residual_out, unit_of(i), u[i]);
       }
     }
+  }
+  // With a norm no registers are left to hold them: L2 fetches them during the row's sum.
+  // 20480 x 3072, nvfp4 / mxfp4: RMSNorm 92 -> 82 / 87 -> 78 us, with the residual
+  // 140 -> 128 / 137 -> 126; asked for before the residual's loads, 139 there.
+  if constexpr (norm_rows(MODE)) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if (active && unit_of(i) < units) {
+        prefetch_l2(p.mod_scale + trow * p.table_stride + unit_of(i) * 16);
+        prefetch_l2(p.shift + trow * p.table_stride + unit_of(i) * 16);
+      }
   }
   uint64_t rinv2 = 0;
   if constexpr (!modulate_only(MODE)) {
@@ -853,14 +891,16 @@ int launch_adaln(Fp4Params p, int format, cudaStream_t stream) {
   if (p.table_stride % 8 != 0 || !aligned16(p.x) || !aligned16(p.shift) ||
       !aligned16(p.mod_scale) || (p.hidden_out != nullptr && !aligned16(p.hidden_out)) ||
       (!modulate_only(MODE) && !aligned16(p.norm_w)) ||
-      (MODE == kResGateRmsModulate &&
+      (has_residual(MODE) &&
        (!aligned16(p.branch) || !aligned16(p.gate) || !aligned16(p.residual_out))))
     return TM_ERR_ALIGNMENT;
   int tpr_log2 = 0, vpt = 0;
   if (!pick_fp4_layout<__nv_bfloat16>(p.cols / 16, &tpr_log2, &vpt)) return TM_ERR_TOO_LARGE;
   // rows are multiples of 64 bytes: 32-byte accesses wherever the tensors start on one
   const auto on32 = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 32 == 0; };
-  const bool wide = on32(p.x) && on32(p.hidden_out) && on32(p.branch) && on32(p.residual_out);
+  bool wide = on32(p.x) && on32(p.hidden_out) && on32(p.branch) && on32(p.residual_out);
+  if (modulate_only(MODE))
+    wide = wide && on32(p.shift) && on32(p.mod_scale) && p.table_stride % 16 == 0;
   return format == TM_FP4_MX
              ? launch_rows<__nv_bfloat16, MODE, kMx>(p, tpr_log2, vpt, wide, stream)
              : launch_rows<__nv_bfloat16, MODE, kNvDynamic>(p, tpr_log2, vpt, wide, stream);
@@ -995,7 +1035,9 @@ int tm_rms_norm_modulate_fp4_quant(uint8_t* q, uint8_t* block_scales, float* sca
   p.norm_w = static_cast<const __nv_bfloat16*>(norm_weight);
   p.eps = eps;
   p.inv_cols = 1.0 / static_cast<double>(cols);
-  return tmw::launch_adaln<tmw::kRmsModulate>(p, format, tmw::as_stream(stream));
+  cudaStream_t st = tmw::as_stream(stream);
+  return index == nullptr ? tmw::launch_adaln<tmw::kRmsModulateRows>(p, format, st)
+                          : tmw::launch_adaln<tmw::kRmsModulate>(p, format, st);
 }
 
 int tm_residual_gate_rms_norm_modulate_fp4_quant(
@@ -1015,7 +1057,9 @@ int tm_residual_gate_rms_norm_modulate_fp4_quant(
   p.branch = static_cast<const __nv_bfloat16*>(branch);
   p.gate = static_cast<const __nv_bfloat16*>(gate);
   p.residual_out = static_cast<__nv_bfloat16*>(residual_out);
-  return tmw::launch_adaln<tmw::kResGateRmsModulate>(p, format, tmw::as_stream(stream));
+  cudaStream_t st = tmw::as_stream(stream);
+  return index == nullptr ? tmw::launch_adaln<tmw::kResGateRmsModulateRows>(p, format, st)
+                          : tmw::launch_adaln<tmw::kResGateRmsModulate>(p, format, st);
 }
 
 }  // extern "C"

@@ -21,7 +21,9 @@ enum QuantMode : int {
   kModulate = 3,   // adaLN modulate, then dynamic
   kRmsModulate = 4,  // RMSNorm, adaLN modulate, then dynamic
   kResGateRmsModulate = 5,  // gated residual add, then as kRmsModulate
-  kModulateRows = 6  // kModulate with one table row per row (no index): tables loaded with x
+  kModulateRows = 6,  // kModulate with one table row per row (no index): tables loaded with x
+  kRmsModulateRows = 7,         // kRmsModulate and kResGateRmsModulate with one table row
+  kResGateRmsModulateRows = 8   // per row: tables asked for before they are used
 };
 
 // adaLN modulate without RMSNorm (indexed or per-row tables)

@@ -231,6 +231,33 @@ def test_producers(tm_ops, cuda, mode, rows, cols, tables, fmt):
         assert again[3] is None and torch.equal(again[0], got[0])
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("shared", [True, False])
+@pytest.mark.parametrize("mode", ["modulate", "rms", "residual"])
+def test_producers_tables_at_16_bytes(tm_ops, cuda, mode, shared, fmt):
+    """Tables that are column slices of a larger tensor, their rows at 16 bytes
+    off a multiple of 32, give the bits of contiguous ones."""
+    rows, cols = 133, 1376
+    g = torch.Generator().manual_seed(5)
+    rnd = lambda *shape: torch.randn(shape, generator=g).bfloat16().to(cuda)  # noqa: E731
+    x, branch, w = rnd(rows, cols), rnd(rows, cols), rnd(cols)
+    sliced = [rnd(4 if shared else rows, cols + 24)[:, 8:cols + 8] for _ in range(3)]
+    index = torch.randint(0, 4, (rows,), generator=g).to(cuda) if shared else None
+
+    def run(shift, scale, gate):
+        if mode == "modulate":
+            return tm_ops.modulate_fp4_quant(x, shift, scale, index, block_format=fmt,
+                                             return_hidden=True)
+        if mode == "rms":
+            return tm_ops.rms_norm_modulate_fp4_quant(x, w, 1e-6, shift, scale, index,
+                                                      block_format=fmt, return_hidden=True)
+        return tm_ops.residual_gate_rms_norm_modulate_fp4_quant(
+            x, branch, gate, w, 1e-6, shift, scale, index, block_format=fmt, return_hidden=True)
+
+    for a, b in zip(run(*sliced), run(*(t.contiguous() for t in sliced)), strict=True):
+        assert (a is None and b is None) or torch.equal(a, b)
+
+
 # ---------------------------------------------------------------- product
 def _operands(tm_ops, cuda, m, n, k, fmt, dtype, seed):
     x = orc.activation(m, k, seed, outlier_channels=None).bfloat16().to(cuda)
