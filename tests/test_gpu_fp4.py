@@ -636,3 +636,29 @@ def test_refusals_on_device_tensors(tm_ops, cuda):
     for call, error in bad:
         with pytest.raises(error):
             call()
+
+
+@pytest.mark.parametrize("tile", [32, 64, 128, 1256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_mm_gelu_is_rounded_once(tm_ops, cuda, dtype, tile):
+    """GELU of exactly known arguments (zero products, so the bias), the negative
+    ones among them, where 1 + tanh cancels.  With t = |2 u| / ln 2 the exponent
+    of exp(-2 u) carries four roundings and the constants' (2^-22 t), the
+    exponential and the reciprocal 2^-22 and 2^-23 (their documented bounds), the
+    sum and the last product 2^-24 each: (t + 2) 2^-22 of the value, and the
+    output's half step."""
+    n = 2048
+    y = torch.linspace(-9.0, 9.0, n, dtype=torch.float64)
+    y[:8] = torch.tensor([-60.0, -20.0, 20.0, 60.0, 0.0, -0.0, -5.5, 1e-3])
+    bias = y.to(dtype)
+    x = tm_ops.scaled_fp4_quant(torch.zeros(5, 64, dtype=dtype, device=cuda))
+    w = tm_ops.scaled_fp4_quant(orc.weight(n, 64, seed=2).to(cuda))
+    out = tm_ops.scaled_mm_fp4(x[0], w[0].t(), x[1], w[1], x[2], w[2], dtype, bias.to(cuda),
+                               gelu_tanh=True, tile=tile).cpu().double()
+    y = bias.double()
+    two_u = 2.0 * (2.0 / torch.pi) ** 0.5 * (y + 0.044715 * y ** 3)
+    ref = y / (1.0 + torch.exp(-two_u))
+    t = two_u.abs() / 0.6931
+    tol = ref.abs() * (HALF_STEP[dtype] * (1 + 2.0 ** -10) + (t + 2) * 2.0 ** -22)
+    tol = tol + y.abs() * 2.0 ** -126 + (2.0 ** -25 if dtype == torch.float16 else 2.0 ** -134)
+    assert ((out - ref).abs() <= tol).all(), ((out - ref).abs() / tol).max()
