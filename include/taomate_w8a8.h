@@ -501,7 +501,10 @@ int tm_dequantize_fp4(void* out, int out_dtype, const uint8_t* q, const uint8_t*
  * The adaLN producers (tm_modulate_int8_quant, tm_rms_norm_modulate_int8_quant,
  * tm_residual_gate_rms_norm_modulate_int8_quant: the same hidden state and
  * residual, bit for bit) followed by tm_scaled_fp4_quant with the row's own
- * scale (`scales`, TM_FP4_NV; NULL for TM_FP4_MX).  cols % 32 == 0, up to 32768;
+ * scale (`scales`, TM_FP4_NV; NULL for TM_FP4_MX).  The norm of a row whose
+ * squares or their sum leave the range of fp32 (values from about 2^63 on, or
+ * below 2^-45 with eps below 2^-60), which the int8 producers do not cover, is
+ * taken from a sum in fp64.  cols % 32 == 0, up to 32768;
  * table_stride % 8 == 0; 16-byte aligned pointers.
  */
 int tm_modulate_fp4_quant(uint8_t* q, uint8_t* block_scales, float* scales, void* hidden_out,

@@ -286,7 +286,7 @@ __device__ __forceinline__ void group_sync(int tpr) {
 
 // Shared words of a block's reductions: a slot per warp for each, written once.
 struct GroupRed {
-  double sum[8];
+  double sum[2][8];
   uint32_t top[8];
 };
 
@@ -305,18 +305,19 @@ __device__ __forceinline__ uint32_t group_max_bits(uint32_t v, int tpr, GroupRed
   return v;
 }
 
-// Sum of one double per thread over the row's group.
-__device__ __forceinline__ double group_sum(double v, int tpr, GroupRed& red) {
+// Sum of one double per thread over the row's group, the same bits in all of its
+// threads; `slots` is red.sum[0] or, for a second sum, red.sum[1].
+__device__ __forceinline__ double group_sum(double v, int tpr, double* slots) {
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
   if (tpr > 32) {
     const int warp = threadIdx.x >> 5;
     const int wpr = tpr >> 5;
     const int first = warp / wpr * wpr;
-    if ((threadIdx.x & 31) == 0) red.sum[warp] = v;
+    if ((threadIdx.x & 31) == 0) slots[warp] = v;
     group_sync(tpr);
-    v = red.sum[first];
-    for (int w = 1; w < wpr; ++w) v += red.sum[first + w];
+    v = slots[first];
+    for (int w = 1; w < wpr; ++w) v += slots[first + w];
   }
   return v;
 }
@@ -445,10 +446,45 @@ __device__ __forceinline__ uint32_t& unit_word(Unit<__nv_bfloat16>& u, int w) {
   return reinterpret_cast<uint32_t*>(u.raw)[w];
 }
 
+// 1 / sqrt(mean of squares + eps) of a row whose squares, or their sum, leave the
+// range of fp32.  They are summed in fp64, where the square of any bf16 value is
+// exact; where the mean itself leaves it, the row is scaled by a power of two
+// (2^-64 or 2^100, in place) and the result belongs to the scaled row, so that the
+// products x * result are those of the row as it was.  Of a row that large, what
+// becomes subnormal is below 2^-125 after the norm.
+template <int VPT>
+__device__ __forceinline__ float row_rms_inverse_f64(const Fp4Params& p,
+                                                     Unit<__nv_bfloat16> (&u)[VPT], bool small,
+                                                     int tpr, GroupRed& red) {
+  double ss = 0.0;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const float2 x = unpack_bf16x2(unit_word(u[i], w));
+      const double lo = x.x, hi = x.y;
+      ss = __fma_rn(hi, hi, __fma_rn(lo, lo, ss));
+    }
+  }
+  const double mean = __dmul_rn(group_sum(ss, tpr, red.sum[1]), p.inv_cols);
+  const double v = mean + static_cast<double>(p.eps);
+  if (v >= 0x1p-100 && v <= 0x1p126)
+    return rsqrt_two_step_rn(__fadd_rn(__double2float_rn(mean), p.eps));
+  const uint32_t factor = small ? 0x71807180u : 0x1f801f80u;  // 2^100, 2^-64 twice
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+#pragma unroll
+    for (int w = 0; w < 8; ++w) unit_word(u[i], w) = bf2_mul(unit_word(u[i], w), factor);
+  }
+  return rsqrt_two_step_rn(__double2float_rn(__dmul_rn(v, small ? 0x1p200 : 0x1p-128)));
+}
+
 // 1 / sqrt(mean of squares + eps) of the row, as the int8 producers compute it:
 // exact fp32 squares added in compensated fp32 chains (TwoSum: every rounding
 // error is kept in a second word), the chains in fp64, then two correctly
-// rounded fp32 steps.
+// rounded fp32 steps.  The squares are exact, and no chain overflows, while their
+// sum is 2^-90 to 2^126 (what vanishes below 2^-149 is then 2^-45 of it at most);
+// a smaller sum beside an eps of 2^-60 or more does not count at all.
 template <int VPT>
 __device__ __forceinline__ float row_rms_inverse(const Fp4Params& p, Unit<__nv_bfloat16> (&u)[VPT],
                                                  int tpr, GroupRed& red) {
@@ -474,7 +510,10 @@ __device__ __forceinline__ float row_rms_inverse(const Fp4Params& p, Unit<__nv_b
     f32x2_split(err[j], e0, e1);
     ss += (static_cast<double>(s0) + e0) + (static_cast<double>(s1) + e1);
   }
-  ss = group_sum(ss, tpr, red);
+  ss = group_sum(ss, tpr, red.sum[0]);
+  const bool small = ss < 0x1p-90;
+  if ((small && p.eps < 0x1p-60f) || !(ss <= 0x1p126))  // overflow leaves an inf or a NaN
+    return row_rms_inverse_f64(p, u, small, tpr, red);
   const float variance = __double2float_rn(__dmul_rn(ss, p.inv_cols));
   return rsqrt_two_step_rn(__fadd_rn(variance, p.eps));
 }

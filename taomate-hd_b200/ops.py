@@ -460,7 +460,8 @@ def rms_norm_modulate_fp4_quant(
     return_hidden: bool = False,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
     """:func:`rms_norm_modulate_int8_quant` with 4-bit output
-    (:func:`modulate_fp4_quant`)."""
+    (:func:`modulate_fp4_quant`).  Rows of any finite values: where their
+    squares leave the range of fp32 the norm is taken from a sum in fp64."""
     _require_cuda(x)
     return _ops.rms_norm_modulate_fp4_quant_new.default(
         x, weight, float(eps), shift, scale, index, _is_mx(block_format), return_hidden)

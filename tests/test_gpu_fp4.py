@@ -662,3 +662,60 @@ def test_mm_gelu_is_rounded_once(tm_ops, cuda, dtype, tile):
     tol = ref.abs() * (HALF_STEP[dtype] * (1 + 2.0 ** -10) + (t + 2) * 2.0 ** -22)
     tol = tol + y.abs() * 2.0 ** -126 + (2.0 ** -25 if dtype == torch.float16 else 2.0 ** -134)
     assert ((out - ref).abs() <= tol).all(), ((out - ref).abs() / tol).max()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-6])
+@pytest.mark.parametrize("rows,cols,tables", [(20, 32, 0), (20, 1376, 3), (20, 5376, 0), (20, 20480, 2)])
+@pytest.mark.parametrize("mode", ["rms", "residual"])
+def test_norm_of_extreme_rows(tm_ops, cuda, mode, rows, cols, tables, eps, fmt):
+    """Rows whose squares leave the range of fp32, beside ordinary ones, against the
+    norm in 64 bits.  Shift and scale are 0, so the hidden state is
+    bf16(x rinv w): rinv carries four fp32 roundings (mean, eps, root, reciprocal),
+    the products two more, 6 2^-24 < 2^-21 of the value; then half a bf16 step, 2^-8.
+    Scaled rows lose at most 2^-134 times 1 / rms <= 2 in their subnormals, and the
+    output as much again: 2^-132."""
+    g = torch.Generator().manual_seed(cols)
+    x = torch.randn((rows, cols), generator=g)
+    power = torch.tensor([0, 60, 62, 63, 64, 70, 100, 120, 125, 0, -30, -40, -45, -50, -60, -64, -70,
+                          -100, -120, -128])
+    x = torch.ldexp(x.clamp(-3.9, 3.9), power.view(-1, 1)).bfloat16()
+    x[9, 1:] *= 2.0 ** -100  # one value carries the row
+    w = (1 + 0.1 * torch.randn(cols, generator=g)).bfloat16()
+    table = torch.zeros(tables or rows, cols, dtype=torch.bfloat16, device=cuda)
+    index = (torch.arange(rows, device=cuda) % tables) if tables else None
+    if mode == "rms":
+        *got, hidden = tm_ops.rms_norm_modulate_fp4_quant(
+            x.to(cuda), w.to(cuda), eps, table, table, index, block_format=fmt, return_hidden=True)
+    else:
+        *got, residual, hidden = tm_ops.residual_gate_rms_norm_modulate_fp4_quant(
+            x.to(cuda), torch.ones_like(x, device=cuda), table, w.to(cuda), eps, table, table, index,
+            block_format=fmt, return_hidden=True)
+        assert torch.equal(residual.cpu(), x)
+    _check_quant(got, hidden.cpu(), fmt)
+    v = x.double()
+    eps = torch.tensor(eps, dtype=torch.float32).double()
+    ref = v / torch.sqrt(v.square().mean(-1, keepdim=True) + eps) * w.double()
+    err = (hidden.cpu().double() - ref).abs()
+    tol = ref.abs() * (2.0 ** -8 + 2.0 ** -21) + 2.0 ** -132
+    assert (err <= tol).all(), (err / tol).amax(-1)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_norm_of_rows_without_a_value(tm_ops, cuda, fmt):
+    """An infinity or a NaN beside huge rows: its row (its block) is NaN, the others'
+    norms are finite; an all-zero row with eps 0 is 0 / 0."""
+    x = torch.randn(6, 64, generator=torch.Generator().manual_seed(2))
+    x[0] *= 2.0 ** 100
+    x[1, 5], x[2, 40], x[3] = float("inf"), float("nan"), 0.0
+    x = x.bfloat16().to(cuda)
+    zero, one = torch.zeros(6, 64, dtype=torch.bfloat16, device=cuda), torch.ones(64, device=cuda).bfloat16()
+    *got, hidden = tm_ops.rms_norm_modulate_fp4_quant(x, one, 0.0, zero, zero, block_format=fmt,
+                                                      return_hidden=True)
+    nan = torch.isnan(hidden.cpu())
+    assert nan[1, 5] and nan[2].all() and nan[3].all() and not nan[[0, 4, 5]].any()
+    assert (hidden[1].cpu()[~nan[1]] == 0).all() and nan[1].sum() == 1
+    _check_quant(got, hidden.cpu(), fmt)
+    *_, hidden = tm_ops.rms_norm_modulate_fp4_quant(x, one, 1e-6, zero, zero, block_format=fmt,
+                                                    return_hidden=True)
+    assert (hidden[3] == 0).all()
