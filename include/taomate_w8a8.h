@@ -476,7 +476,8 @@ int tm_fp4_block_scales_size(int64_t rows, int64_t cols, int format, uint64_t* b
  *   TM_FP4_MX  s = 2^(floor(log2 m) - 2), at least 2^-127;  q = e2m1(x / s)
  * Each quotient is rounded once, from its exact value, to nearest (ties to
  * even), q to at most 6.  Exactly one of scales and given_scale is non-NULL for
- * TM_FP4_NV, neither for TM_FP4_MX.  given_scale must be positive, from 2^-110 to 2^110.
+ * TM_FP4_NV, neither for TM_FP4_MX.  given_scale must lie from 2^-110 to 2^110; with
+ * any other value (0, a NaN) every block gets the scale NaN and codes 0.
  * A row with an inf or a NaN gets the outer scale NaN, block scales and codes 0;
  * where there is no outer scale to be written, such a block gets the scale NaN and
  * codes 0: either way the products with it are NaN.

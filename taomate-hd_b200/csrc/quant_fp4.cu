@@ -327,7 +327,8 @@ struct RowScale {
   float o;      // outer scale (TM_FP4_NV)
   float inv6o;  // 1 / (6 o) to 2^-22
   float nudge;  // 1 +- 2^-20 (above); 0: the general way
-  bool bad;     // the row holds an inf or a NaN (its own scale is NaN, blocks and codes 0)
+  bool bad;     // the row holds an inf or a NaN (its own scale is NaN, blocks and codes 0);
+                // or the given scale is out of range (block scales NaN, codes 0)
 };
 
 __device__ __forceinline__ RowScale row_scale(uint32_t max_bits) {
@@ -342,8 +343,11 @@ __device__ __forceinline__ RowScale row_scale(uint32_t max_bits) {
   return r;
 }
 
+// From 2^-110 to 2^110 every product of o with a code, a block scale and a border is
+// a normal fp32 number.  Others (a scale of 0, say, or a NaN) are refused where they
+// can be seen without a copy to the host: here, by NaN for the whole tensor.
 __device__ __forceinline__ RowScale given_scale(float o) {
-  return RowScale{o, rcp_approx(__fmul_rn(6.0f, o)), 0.0f, false};
+  return RowScale{o, rcp_approx(__fmul_rn(6.0f, o)), 0.0f, !(o >= 0x1p-110f && o <= 0x1p110f)};
 }
 
 // Convert one unit (16 elements, block maximum `m_bits` as fp32 bits) and
@@ -366,7 +370,7 @@ __device__ __forceinline__ uint32_t convert_unit(const Unit<T>& u, uint32_t m_bi
     }
     return byte;
   } else {
-    if (KIND == kNvGiven && m_bits >= kInfBits) return 0x7fu;  // e4m3 NaN
+    if (KIND == kNvGiven && (m_bits >= kInfBits || rs.bad)) return 0x7fu;  // e4m3 NaN
     if (rs.bad) return 0u;
     if (KIND == kNvDynamic && sizeof(T) == 2 && rs.nudge != 0.0f) {  // the same for the whole row
       const float z = __fmul_rn(__uint_as_float(m_bits), __fmul_rn(rs.inv6o, rs.nudge));

@@ -209,8 +209,9 @@ def scaled_fp4_quant(
 
     * ``"nvfp4"``: blocks of 16 with an e4m3 scale, times an fp32 scale of
       each row (``scales``, ``[rows, 1]``), or of the whole tensor when
-      ``scale`` (one fp32 value, the step between stored and real values) is
-      given; ``scales`` is then that tensor.
+      ``scale`` (one fp32 value from 2^-110 to 2^110, the step between stored
+      and real values) is given; ``scales`` is then that tensor.  The value is
+      not copied to the host: one out of range makes the whole tensor NaN.
     * ``"mxfp4"``: blocks of 32 with a power-of-two scale (e8m0); ``scales``
       is ``None`` and no ``scale`` is taken.
 

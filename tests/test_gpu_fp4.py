@@ -719,3 +719,31 @@ def test_norm_of_rows_without_a_value(tm_ops, cuda, fmt):
     *_, hidden = tm_ops.rms_norm_modulate_fp4_quant(x, one, 1e-6, zero, zero, block_format=fmt,
                                                     return_hidden=True)
     assert (hidden[3] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("power", [-110, 110])
+def test_given_scale_at_the_ends_of_its_range(tm_ops, cuda, dtype, power):
+    given = 2.0 ** power
+    x = torch.cat((_borders(dtype).double() * given, _borders(dtype).double() * given * 2.0 ** -9,
+                   _borders(dtype).double() * 2.0 ** (power // 2))).to(dtype)
+    got = tm_ops.scaled_fp4_quant(x.to(cuda), torch.tensor([given], device=cuda))
+    _check_quant(got, x, "nvfp4", given)
+
+
+@pytest.mark.parametrize("given", [0.0, -0.0, -1.0, float("nan"), float("inf"), 2.0 ** -111, 2.0 ** 111])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_given_scale_out_of_range_is_nan(tm_ops, cuda, dtype, given):
+    """Every block scale is NaN and every code 0, in all-zero blocks too; the padding
+    stays 0."""
+    scale = torch.tensor([given], device=cuda)
+    big = torch.randn(131, 33024, generator=torch.Generator().manual_seed(1)).to(dtype).to(cuda)
+    big[3] = 0.0
+    for x in (big[:, :96], big[:, 1:97], big[:2]):  # both kernels
+        q, blocks, _ = tm_ops.scaled_fp4_quant(x, scale)
+        rows, cols = x.shape
+        want = np.zeros(blocks.numel(), dtype=np.uint8)
+        want[f4.tile_offsets(rows, cols // 16)] = 0x7F
+        np.testing.assert_array_equal(blocks.view(torch.uint8).cpu().numpy().reshape(-1), want)
+        assert not q.any()
+        assert torch.isnan(tm_ops.dequantize_fp4(q, blocks, scale)).all()
