@@ -181,7 +181,7 @@ template <typename OutT>
 __device__ __forceinline__ RowConsts row_consts(const Fp4Args& g, int n) {
   RowConsts c{n, 1.f, 0.f};
   if (n < g.N) {
-    if (g.sb != nullptr) c.sb = __ldg(g.sb + (g.sb_per_col ? n : 0));
+    if (g.sb != nullptr) c.sb = ld_nc_f32(g.sb + (g.sb_per_col ? n : 0));
     if (g.bias != nullptr) c.bias = out_to_f32<OutT>(static_cast<const OutT*>(g.bias)[n]);
   }
   return c;
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(kSmallThreads)
     const RowConsts c = row_consts<OutT>(g, nb * kTileRows + row);
     if (threadIdx.x - 64 < TOK) {
       const int t = threadIdx.x - 64;
-      token_sa[t] = g.sa == nullptr || t >= tokens ? 1.f : __ldg(g.sa + (g.sa_per_row ? m0 + t : 0));
+      token_sa[t] = g.sa == nullptr || t >= tokens ? 1.f : ld_nc_f32(g.sa + (g.sa_per_row ? m0 + t : 0));
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");  // the epilogue warps: token_sa is complete
     const bool ok = mbar_wait_warp(bar.acc, 0, bar.abort_flag, g.status);
@@ -556,11 +556,11 @@ __device__ __forceinline__ PairConsts pair_consts(const Fp4Args& g, int nb, int 
   const bool in = col < g.N;  // N % 8 == 0: all four or none
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    c.sb[j] = FORMAT == TM_FP4_NV && in ? __ldg(g.sb + (g.sb_per_col ? col + j : 0)) : 0.f;
+    c.sb[j] = FORMAT == TM_FP4_NV && in ? ld_nc_f32(g.sb + (g.sb_per_col ? col + j : 0)) : 0.f;
     c.bias[j] =
         g.bias != nullptr && in ? out_to_f32<OutT>(static_cast<const OutT*>(g.bias)[col + j]) : 0.f;
   }
-  c.sa = FORMAT == TM_FP4_NV && row < g.M ? __ldg(g.sa + (g.sa_per_row ? row : 0)) : 1.f;
+  c.sa = FORMAT == TM_FP4_NV && row < g.M ? ld_nc_f32(g.sa + (g.sa_per_row ? row : 0)) : 1.f;
   return c;
 }
 

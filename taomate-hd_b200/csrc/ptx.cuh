@@ -125,6 +125,20 @@ __device__ __forceinline__ void griddep_wait() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// To the compiler the data of a read-only load (`__ldg`) never changes: it may move
+// one ahead of griddep_wait.  What the grid before may have written is read by plain
+// loads, by volatile ones, or from an address that depends on an index only known
+// behind the wait.
+__device__ __forceinline__ int behind_wait(int index) {
+  asm volatile("" : "+r"(index)::"memory");
+  return index;
+}
+__device__ __forceinline__ float ld_nc_f32(const float* p) {
+  float v;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+
 __device__ __forceinline__ void griddep_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }

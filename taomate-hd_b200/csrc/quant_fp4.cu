@@ -182,6 +182,14 @@ __device__ __forceinline__ uint32_t scaled_codes8(const float (&x)[8], float inv
   return e2m1x8(a);
 }
 
+__device__ __forceinline__ uint4 ld_nc_u32x4(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
 // 32 bytes that no kernel in flight writes; `wide`: the address is a multiple of
 // 32 (one load), else of 16.  Volatile, so that it stays behind griddep_wait(); the
 // loads of an unrolled loop are still issued ahead of its stores (timed: no difference).
@@ -192,8 +200,8 @@ __device__ __forceinline__ void ld_stream32(const void* p, bool wide, uint4& a, 
                    "=r"(b.w)
                  : "l"(p));
   } else {
-    a = ld_cached16(p);
-    b = ld_cached16(static_cast<const uint8_t*>(p) + 16);
+    a = ld_nc_u32x4(p);
+    b = ld_nc_u32x4(static_cast<const uint8_t*>(p) + 16);
   }
 }
 
@@ -205,8 +213,8 @@ __device__ __forceinline__ void ld_table32(const void* p, bool wide, uint4& a, u
                    "=r"(b.w)
                  : "l"(p));
   } else {
-    a = ld_cached16(p);
-    b = ld_cached16(static_cast<const uint8_t*>(p) + 16);
+    a = ld_nc_u32x4(p);
+    b = ld_nc_u32x4(static_cast<const uint8_t*>(p) + 16);
   }
 }
 
@@ -680,7 +688,7 @@ __global__ void __launch_bounds__(256, (fp4_min_blocks<T, VPT, MODE>())) quant_f
     rs = row_scale(group_max_bits(top, tpr, red));
     if (active && t == 0) p.scales[row] = rs.o;
   } else if constexpr (KIND == kNvGiven) {
-    rs = given_scale(__ldg(p.static_scale));
+    rs = given_scale(ld_nc_f32(p.static_scale));
   }
   if (row >= p.padded_rows) return;
   const RowOut out = row_out(p, row);
@@ -722,7 +730,7 @@ __global__ void __launch_bounds__(256) quant_fp4_any_kernel(const Fp4Params p) {
     rs = row_scale(group_max_bits(top, 256, red));
     if (active && threadIdx.x == 0) p.scales[row] = rs.o;
   } else if constexpr (KIND == kNvGiven) {
-    rs = given_scale(__ldg(p.static_scale));
+    rs = given_scale(ld_nc_f32(p.static_scale));
   }
   const RowOut out = row_out(p, row);
   const int lane_units = (pad_units + 255) / 256 * 256;  // whole warps: shuffles below
@@ -805,14 +813,17 @@ __global__ void __launch_bounds__(256) dequant_fp4_kernel(const DequantParams p)
   griddep_wait();
   griddep_launch_dependents();
   const int tpr = 1 << p.tpr_log2;
-  const int t = threadIdx.x & (tpr - 1);
+  // read-only loads, which the unrolled loop may issue ahead of its stores: every
+  // address depends on a row that is only known behind the wait
+  const int thread = behind_wait(static_cast<int>(threadIdx.x));
+  const int t = thread & (tpr - 1);
   const int64_t row =
-      static_cast<int64_t>(blockIdx.x) * (blockDim.x >> p.tpr_log2) + (threadIdx.x >> p.tpr_log2);
+      static_cast<int64_t>(blockIdx.x) * (blockDim.x >> p.tpr_log2) + (thread >> p.tpr_log2);
   if (row >= p.rows) return;
   const int units = static_cast<int>(p.cols / 16);
   const uint8_t* blocks = p.blocks + fp4_scale_offset(row, 0, p.ktiles);
   const uint2* codes = reinterpret_cast<const uint2*>(p.codes + row * (p.cols / 2));
-  const float o = p.scales == nullptr ? 1.0f : __ldg(p.scales + (p.per_row ? row : 0));
+  const float o = p.scales == nullptr ? 1.0f : ld_nc_f32(p.scales + (p.per_row ? row : 0));
   T* out = static_cast<T*>(p.out) + row * p.cols;
 #pragma unroll 4
   for (int unit = t; unit < units; unit += tpr) {

@@ -160,3 +160,24 @@ def test_python_refusals():
         ops._is_mx("fp4")
     with pytest.raises(NotImplementedError):  # no CPU implementation is registered
         torch.ops.taomate_w8a8.scaled_fp4_quant_new(x, None, False)
+
+
+@pytest.mark.parametrize("name", ["quant_fp4.cu", "gemm_fp4.cu"])
+def test_reads_stay_behind_the_wait_for_the_previous_grid(name):
+    """The kernels start while the grid before them runs, so no load of its results may
+    be one that the compiler can move ahead of griddep_wait: a kernel with read-only
+    loads takes its thread index, on which every address depends, from behind the wait,
+    and the load helpers' assembly is volatile."""
+    import re
+    from pathlib import Path
+
+    csrc = Path(capi_mod.__file__).parent / "csrc"
+    source = (csrc / name).read_text()
+    for part in source.split("__global__"):
+        if re.search(r"__ldg\(|ld_cached16\(|ld_nc16\(", part):
+            assert part.count("threadIdx") == 1
+            assert part.index("griddep_wait();") < part.index("behind_wait(static_cast<int>(threadIdx.x))")
+    text = source + "".join((csrc / h).read_text() for h in ("ptx.cuh", "rows.cuh"))
+    for helper in set(re.findall(r"\b(ld_\w+|prefetch_\w+)\(", source)):
+        body = re.search(rf"\b{helper}\([^)]*\)\s*{{(.*?)\n}}", text, re.S)
+        assert body and not re.search(r"asm\(", body[1]), helper
