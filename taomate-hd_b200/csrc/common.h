@@ -51,6 +51,20 @@ bool allow_smem(Kernel kernel, int bytes, int device, std::atomic<bool> (&done)[
   return true;
 }
 
+// A positive number that `query` finds for each device, asked for by any host
+// thread and kept in `known` (a static array of the call site).  A query that
+// fails (0) is not kept: the next call asks again.  Losing a race repeats it.
+template <typename Query>
+int known_per_device(std::atomic<int> (&known)[64], int device, Query query) {
+  if (device < 0 || device >= 64) return 0;
+  int n = known[device].load(std::memory_order_acquire);
+  if (n > 0) return n;
+  n = query();
+  if (n <= 0) return 0;
+  known[device].store(n, std::memory_order_release);
+  return n;
+}
+
 // Launch with programmatic dependent launch allowed (the kernel calls
 // griddep_wait before reading global data): `attrs` are the launch's other
 // attributes.  Should the driver refuse the combination, the launch is

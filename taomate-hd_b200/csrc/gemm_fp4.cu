@@ -955,31 +955,31 @@ int launch_small(const Fp4Operand& x, const Fp4Operand& w, Fp4Args args, int spl
 // Resident pairs of the pair kernel on a device (cached; its instances differ by
 // a few KiB of shared memory only, one CTA an SM each).
 int max_fp4_pairs(int device, int sms) {
-  static int cache[64] = {};
-  if (device < 0 || device >= 64) return 0;
-  if (cache[device] == 0) {
+  static std::atomic<int> known[64] = {};
+  return known_per_device(known, device, [&] {
     auto kernel = gemm_fp4_pair_kernel<TM_FP4_NV, 0, __nv_bfloat16>;
     constexpr int smem = PairLayout<TM_FP4_NV>::kTotal;
+    cudaError_t err =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(sms & ~1));
+    cfg.blockDim = dim3(kPairThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
     int clusters = 0;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) ==
-        cudaSuccess) {
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(static_cast<unsigned>(sms & ~1));
-      cfg.blockDim = dim3(kPairThreads);
-      cfg.dynamicSmemBytes = smem;
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = 2;
-      attr[0].val.clusterDim.y = 1;
-      attr[0].val.clusterDim.z = 1;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) clusters = 0;
+    if (err == cudaSuccess) err = cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg);
+    if (err != cudaSuccess) {
+      cudaGetLastError();  // a failed query must not poison later launches
+      return 0;
     }
-    cudaGetLastError();  // a failed query must not poison later launches
-    cache[device] = clusters > 0 ? clusters : -1;
-  }
-  return cache[device] > 0 ? cache[device] : 0;
+    return clusters;
+  });
 }
 
 template <int FORMAT, int EPI, typename OutT>

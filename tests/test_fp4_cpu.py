@@ -181,3 +181,52 @@ def test_reads_stay_behind_the_wait_for_the_previous_grid(name):
     for helper in set(re.findall(r"\b(ld_\w+|prefetch_\w+)\(", source)):
         body = re.search(rf"\b{helper}\([^)]*\)\s*{{(.*?)\n}}", text, re.S)
         assert body and not re.search(r"asm\(", body[1]), helper
+
+
+def test_device_numbers_are_kept_only_once_known(tmp_path):
+    """known_per_device (the resident pairs of the 4-bit product): a failed query is
+    asked again, a found number is kept for its device, other devices and numbers out of
+    range do not touch it, and host threads may ask at once (thread sanitiser)."""
+    import shutil
+    import subprocess
+    from pathlib import Path
+
+    from taomate_hd_b200 import build
+
+    csrc = Path(capi_mod.__file__).parent / "csrc"
+    source = (csrc / "gemm_fp4.cu").read_text()
+    body = source[source.index("int max_fp4_pairs("):]
+    assert "known_per_device(" in body[:body.index("\n}\n")] and "static int cache" not in source
+    (tmp_path / "t.cpp").write_text(f"""
+#include <cassert>
+#include <thread>
+#include <vector>
+#include "{csrc / 'common.h'}"
+int main() {{
+  static std::atomic<int> known[64] = {{}};
+  int asked = 0;
+  auto fails = [&] {{ ++asked; return 0; }};
+  assert(tmw::known_per_device(known, 3, fails) == 0);
+  assert(tmw::known_per_device(known, 3, fails) == 0 && asked == 2);
+  auto seven = [&] {{ ++asked; return 7; }};
+  assert(tmw::known_per_device(known, 3, seven) == 7 && asked == 3);
+  assert(tmw::known_per_device(known, 3, fails) == 7 && asked == 3);
+  assert(tmw::known_per_device(known, 4, fails) == 0 && asked == 4);
+  assert(tmw::known_per_device(known, -1, seven) == 0 && tmw::known_per_device(known, 64, seven) == 0);
+  std::vector<std::thread> all;
+  for (int i = 0; i < 8; ++i)
+    all.emplace_back([&] {{
+      for (int d = 0; d < 64; ++d)
+        assert(tmw::known_per_device(known, d, [&] {{ return 7; }}) == 7);
+    }});
+  for (auto& t : all) t.join();
+}}
+""")
+    compiler = shutil.which("g++")
+    assert compiler
+    command = [compiler, "-std=c++17", "-O1", f"-I{build._cuda_home() / 'include'}", "-pthread",
+               str(tmp_path / "t.cpp"), "-o", str(tmp_path / "t")]
+    sanitised = subprocess.run([*command, "-fsanitize=thread"], capture_output=True, text=True)
+    if sanitised.returncode:  # no sanitiser runtime on this machine
+        subprocess.run(command, check=True)
+    subprocess.run([str(tmp_path / "t")], check=True, timeout=120)
