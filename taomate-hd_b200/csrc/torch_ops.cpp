@@ -768,7 +768,7 @@ Fp4Result scaled_fp4_quant_new(const at::Tensor& input, const std::optional<at::
   const bool rows = input.dim() == 2 && input.stride(1) == 1 &&
                     (input.size(0) <= 1 || input.stride(0) >= input.size(1));
   scaled_fp4_quant(t.q, t.blocks, t.scales, rows ? input : input.contiguous(), scale);
-  return {t.q, t.blocks, scale.has_value() ? scale : t.scales};
+  return {t.q, t.blocks, t.scales};  // none where a scale is given: the schema's outputs are fresh
 }
 
 at::Tensor dequantize_fp4_new(const at::Tensor& q, const at::Tensor& block_scales,

@@ -221,7 +221,8 @@ def scaled_fp4_quant(
     infinity or a NaN becomes NaN as a whole.
     """
     _require_cuda(input)
-    return _scaled_fp4_quant(input, scale, _is_mx(block_format))
+    q, block_scales, scales = _scaled_fp4_quant(input, scale, _is_mx(block_format))
+    return q, block_scales, scales if scale is None else scale
 
 
 def dequantize_fp4(

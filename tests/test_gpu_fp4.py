@@ -747,3 +747,39 @@ def test_given_scale_out_of_range_is_nan(tm_ops, cuda, dtype, given):
         np.testing.assert_array_equal(blocks.view(torch.uint8).cpu().numpy().reshape(-1), want)
         assert not q.any()
         assert torch.isnan(tm_ops.dequantize_fp4(q, blocks, scale)).all()
+
+
+def test_allocating_operators_return_fresh_tensors(tm_ops, cuda):
+    """The operators' outputs share no storage with an input, as their schemas say, a
+    given scale among them; the Python call hands the given scale back itself."""
+    raw = torch.ops.taomate_w8a8
+    x = torch.randn(6, 64, device=cuda).bfloat16()
+    scale = torch.tensor([0.01], device=cuda)
+    w = tm_ops.scaled_fp4_quant(torch.randn(8, 64, device=cuda))
+    q, b, s = tm_ops.scaled_fp4_quant(x)
+    one = torch.ones(64, device=cuda).bfloat16()
+
+    def check(op, args):
+        outs = op.default(*args)
+        storages = lambda ts: [t.untyped_storage().data_ptr() for t in ts  # noqa: E731
+                               if isinstance(t, torch.Tensor)]
+        outs = storages(outs if isinstance(outs, tuple) else (outs,))
+        assert len(set(outs)) == len(outs) and not set(outs) & set(storages(args))
+
+    check(raw.scaled_fp4_quant_new, (x, None, False))
+    check(raw.scaled_fp4_quant_new, (x, None, True))
+    check(raw.scaled_fp4_quant_new, (x, scale, False))
+    assert raw.scaled_fp4_quant_new(x, scale, False)[2] is None
+    # torch's own check of the schema (it takes no 8-bit floating-point inputs)
+    torch.library.opcheck(raw.scaled_fp4_quant_new.default, (x, scale, False),
+                          test_utils="test_schema")
+    check(raw.dequantize_fp4_new, (q, b, s, torch.bfloat16))
+    check(raw.scaled_mm_fp4_new, (q, w[0].t(), b, w[1], s, w[2], torch.bfloat16, None, 0))
+    check(raw.modulate_fp4_quant_new, (x, x, x, None, False, True))
+    check(raw.rms_norm_modulate_fp4_quant_new, (x, one, 1e-6, x, x, None, False, True))
+    check(raw.residual_gate_rms_norm_modulate_fp4_quant_new,
+          (x, x, x, one, 1e-6, x, x, None, False, True))
+    got = tm_ops.scaled_fp4_quant(x, scale)
+    assert got[2] is scale
+    y = tm_ops.scaled_mm_fp4(got[0], w[0].t(), got[1], w[1], got[2], w[2])
+    _check_mm(y, *got, *w, None, "nvfp4")
