@@ -262,8 +262,9 @@ def scaled_mm_fp4(
     mxfp4).  ``N`` must be a multiple of 8.  ``gelu_tanh`` and ``swiglu``
     (interleaved gate/up rows, :func:`interleave_gate_up`) as in
     :func:`scaled_mm`, except that the result is rounded once, after the
-    activation.  ``out`` ([M, N] or [M, N / 2]) makes the call allocation-free;
-    ``tile`` and ``splits`` force a kernel configuration (0 = heuristic).
+    activation.  ``out`` ([M, N] or [M, N / 2], its dtype in place of ``out_dtype``)
+    makes the call allocation-free; ``tile`` and ``splits`` force a kernel
+    configuration (tile 0 = heuristic, which chooses the splits too).
     """
     _require_cuda(a)  # the operator checks that the others are on its device
     if gelu_tanh and swiglu:
@@ -273,12 +274,13 @@ def scaled_mm_fp4(
         return _scaled_mm_fp4(a, b, block_scale_a, block_scale_b, scale_a, scale_b, out_dtype, bias,
                               epi)
     a2 = a.reshape(-1, a.shape[-1])
-    if out is None:
+    y = out
+    if y is None:
         cols = b.shape[1] // 2 if swiglu else b.shape[1]
-        out = torch.empty((a2.shape[0], cols), dtype=out_dtype, device=a.device)
-    _ops.scaled_mm_fp4.default(out, a2, b, block_scale_a, block_scale_b, scale_a, scale_b, bias,
+        y = torch.empty((a2.shape[0], cols), dtype=out_dtype, device=a.device)
+    _ops.scaled_mm_fp4.default(y, a2, b, block_scale_a, block_scale_b, scale_a, scale_b, bias,
                                epi, tile, splits)
-    return out
+    return y if out is not None else y.view(*a.shape[:-1], y.shape[1])
 
 
 def quantize_weight_int8(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

@@ -783,3 +783,23 @@ def test_allocating_operators_return_fresh_tensors(tm_ops, cuda):
     assert got[2] is scale
     y = tm_ops.scaled_mm_fp4(got[0], w[0].t(), got[1], w[1], got[2], w[2])
     _check_mm(y, *got, *w, None, "nvfp4")
+
+
+@pytest.mark.parametrize("tile,splits", [(0, 1), (32, 2), (128, 1), (1256, 1)])
+def test_mm_leading_dimensions_under_every_tile(tm_ops, cuda, tile, splits):
+    """[..., K / 2] codes give [..., N] whatever the kernel; `out` is returned as it is."""
+    x = orc.activation(24, 512, 1, outlier_channels=None).bfloat16().to(cuda).view(2, 3, 4, 512)
+    q, b, s = tm_ops.scaled_fp4_quant(x)
+    w = tm_ops.scaled_fp4_quant(orc.weight(128, 512, seed=2).to(cuda))
+    for swiglu, n in ((False, 128), (True, 64)):
+        y = tm_ops.scaled_mm_fp4(q, w[0].t(), b, w[1], s, w[2], swiglu=swiglu, tile=tile,
+                                 splits=splits)
+        assert y.shape == (2, 3, 4, n)
+        _check_mm(y.view(24, n), q.view(24, -1), b, s, *w, None, "nvfp4", "swiglu" if swiglu else "none")
+        out = torch.empty(24, n, dtype=torch.bfloat16, device=cuda)
+        assert tm_ops.scaled_mm_fp4(q, w[0].t(), b, w[1], s, w[2], swiglu=swiglu, out=out, tile=tile,
+                                    splits=splits) is out
+        assert torch.equal(out, y.view(24, n))
+    empty = tm_ops.scaled_fp4_quant(x[:0])
+    assert tm_ops.scaled_mm_fp4(empty[0], w[0].t(), empty[1], w[1], empty[2], w[2], tile=tile,
+                                splits=splits).shape == (0, 3, 4, 128)
