@@ -803,3 +803,49 @@ def test_mm_leading_dimensions_under_every_tile(tm_ops, cuda, tile, splits):
     empty = tm_ops.scaled_fp4_quant(x[:0])
     assert tm_ops.scaled_mm_fp4(empty[0], w[0].t(), empty[1], w[1], empty[2], w[2], tile=tile,
                                 splits=splits).shape == (0, 3, 4, 128)
+
+
+def _device_values(q, b, s, fmt):
+    """_values for large tensors: the same by torch operations on the device."""
+    rows, blocks = q.shape[0], q.shape[1] * 2 // f4.BLOCK[fmt]
+    code = torch.stack((q & 15, q >> 4), -1).view(rows, blocks, -1).long()
+    value = torch.tensor(np.concatenate((f4.E2M1, -f4.E2M1)), device=q.device)[code]
+    at = torch.from_numpy(f4.tile_offsets(rows, blocks)).to(q.device)
+    v = (value * b.float().double().view(-1)[at].unsqueeze(-1)).view(rows, -1)
+    return (v if s is None else v * s.double().view(-1, 1)).cpu().numpy()
+
+
+def _large_mm(tm_ops, cuda, monkeypatch, m, n, k, fmt, act, **forced):
+    monkeypatch.setitem(globals(), "_values", _device_values)
+    g = torch.Generator(device=cuda).manual_seed(m + n + k)
+    rnd = lambda *shape: torch.randn(shape, generator=g, device=cuda)  # noqa: E731
+    a = tm_ops.scaled_fp4_quant(rnd(m, k).bfloat16(), block_format=fmt)
+    w = tm_ops.scaled_fp4_quant((rnd(n, k) * 0.03).bfloat16(), block_format=fmt)
+    bias = (rnd(n) * 0.3).bfloat16()
+    out = tm_ops.scaled_mm_fp4(a[0], w[0].t(), a[1], w[1], a[2], w[2], bias=bias,
+                               gelu_tanh=act == "gelu", swiglu=act == "swiglu", **forced)
+    _check_mm(out, *a, *w, bias, fmt, act)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("act", ["none", "gelu", "swiglu"])
+@pytest.mark.parametrize("m,n,k", [
+    (1, 20032, 2336), (33, 20032, 288), (128, 24000, 1056), (5, 40000, 544), (64, 19008, 96),
+    (256, 9472, 608), (256, 9536, 608),   # 148 tiles of 128 x 128, and 150
+    (129, 18944, 416), (1000, 2368, 800), (1000, 2432, 800),
+])
+def test_mm_more_tiles_than_sms(tm_ops, cuda, monkeypatch, m, n, k, act, fmt):
+    """The chosen kernel where the small one has more tiles than the GPU has SMs (two
+    blocks an SM, shorter rings), and on both sides of the change to the pair kernel."""
+    _large_mm(tm_ops, cuda, monkeypatch, m, n, k, fmt, act)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tile,splits,m,n,k", [
+    (32, 8, 20, 4160, 2336), (32, 2, 32, 12800, 800), (64, 4, 64, 8256, 1376), (128, 2, 300, 4160, 800),
+    (128, 8, 300, 1344, 2336), (128, 4, 128, 6400, 1056),
+])
+def test_mm_slices_of_more_tiles_than_sms(tm_ops, cuda, monkeypatch, tile, splits, m, n, k, fmt):
+    """Clusters of K slices in several waves, where two stages may exceed half an SM."""
+    for act in ("none", "swiglu"):
+        _large_mm(tm_ops, cuda, monkeypatch, m, n, k, fmt, act, tile=tile, splits=splits)
