@@ -612,11 +612,11 @@ __device__ __forceinline__ void pair_finish16(uint32_t* r, uint64_t sa2, bool ha
 
 // Store 16 columns of this lane's row, as one 32-byte sector where the output
 // allows it (`wide`: rows start on 32-byte boundaries).  8192 x 12288 x 3072
-// nvfp4: two 16-byte stores in place of the one cost 197 against 150 us; staged
-// TMA stores (121 against 123), or full lines after an exchange between lanes
-// (mxfp4 117 against 111), gain nothing: what remains is the output's share of
-// the traffic.
-// Not allocating in L1: with GELU 134 -> 129 us.
+// nvfp4: two 16-byte stores in place of the one cost 154 against 130 us, with GELU
+// 162 against 143; staged TMA stores (121 against 123 when they were tried), or full
+// lines after an exchange between lanes (mxfp4 117 against 111), gain nothing: what
+// remains is the output's share of the traffic.
+// Not allocating in L1: 135 -> 130 us, with GELU 148 -> 143.
 template <typename OutT>
 __device__ __forceinline__ void pair_store16(OutT* row, const uint32_t* y, int col, int cols,
                                              bool wide) {
@@ -1027,17 +1027,17 @@ struct Fp4Choice {
 };
 
 // Measured on a B200 (back to back, us): one wave of 128 x 128 tiles is ahead of
-// the pair kernel (512 x 3072 x 3072: 7.6 against 10.3; 1003 x 1160 x 1376: 6.9
-// against 9.8), two waves are level or behind (1024 x 3072 x 3072: 10.3 against
-// 10.7; 256 x 12288 x 3072: 11.5 against 10.9; 512 x 12288 x 3072: 18.9 against
-// 16.6), so more than 128 tokens take the small kernel only while its tiles fit the
-// SMs at once.  Up to 128 tokens the weight is read once either way, by twice the
-// CTAs (128 x 12288 x 3072: 8.5 against 10.8).
+// the pair kernel (512 x 3072 x 3072: 7.6 against 8.9; 1003 x 1160 x 1376: 6.8
+// against 9.6), two waves are behind (1024 x 3072 x 3072: 10.3 against 9.5; with GELU
+// 256 x 12288 x 3072: 12.0 against 11.1, 512 x 12288 x 3072: 19.5 against 15.3), so
+// more than 128 tokens take the small kernel only while its tiles fit the SMs at
+// once.  Up to 128 tokens the weight is read once either way, by twice the CTAs (128 x
+// 12288 x 3072: 7.9 against 9.5, with GELU 9.0 against 11.0).
 //
 // Slices of K: about 0.2 us a k-block, against 0.7 us and what grows with the
 // slices and tokens for the partial sums; only while every slice has an SM of its
-// own (1 x 3072 x 12288: 12.3, 7.5, 6.2 us with 1, 2, 4 slices; 48 x 3072 x 12288
-// mxfp4: 12.5, 8.8, 6.9; 256 x 3072 x 3072: 7.1, 8.8, 13.7).
+// own (1 x 3072 x 12288: 12.4, 7.6, 6.2 us with 1, 2, 4 slices; 48 x 3072 x 12288
+// mxfp4: 12.5, 8.9, 7.0; 256 x 3072 x 3072: 7.1, 8.8, 13.7).
 Fp4Choice pick_fp4(int64_t m, int64_t n, int kblocks, const Fp4Device& dev) {
   Fp4Choice c{m <= 32 ? 32 : m <= 64 ? 64 : 128, 1};
   const int64_t tiles = (m + c.tile - 1) / c.tile * ((n + kTileRows - 1) / kTileRows);

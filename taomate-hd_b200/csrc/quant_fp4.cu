@@ -27,7 +27,7 @@
 // exactly (t s has at most 7 bits, so the product is not rounded before the
 // subtraction).  The scale's rounding is decided the same way, with its border
 // t: m - (6 t) o.  Taken for every row, 20480 x
-// 3072 bf16 needed 37 us in place of 31.
+// 3072 bf16 needs 36 us in place of 30; with a given scale it is 33.
 //
 // The kernels are bound by HBM: 2 bytes read and 0.56 written per bf16 element.
 // As in the int8 kernels a group of 32..256 threads owns a row and holds it in
@@ -549,7 +549,8 @@ __device__ __forceinline__ void adaln_units(const Fp4Params& p, Unit<__nv_bfloat
   const int64_t trow = active ? (p.index ? p.index[row] : row) : 0;
   const auto unit_of = [&](int i) { return t + i * tpr; };
   // 32-byte table loads in the producers without a norm: 41 -> 39 us (nvfp4) and 37 -> 34
-  // (mxfp4) at 20480 x 3072 with five tables; with a norm they change nothing (70, 66 us).
+  // (mxfp4) at 20480 x 3072 with five tables; with a norm they change nothing (67, 61 us)
+  // and cost with the residual (94 -> 97, 89 -> 92).
   const auto load = [&](U& v, const __nv_bfloat16* at, int unit) {
     ld_table32(at + unit * 16, wide && modulate_only(MODE), v.raw[0], v.raw[1]);
   };
@@ -589,8 +590,8 @@ __device__ __forceinline__ void adaln_units(const Fp4Params& p, Unit<__nv_bfloat
     }
   }
   // With a norm no registers are left to hold them: L2 fetches them during the row's sum.
-  // 20480 x 3072, nvfp4 / mxfp4: RMSNorm 92 -> 82 / 87 -> 78 us, with the residual
-  // 140 -> 128 / 137 -> 126; asked for before the residual's loads, 139 there.
+  // 20480 x 3072, nvfp4 / mxfp4: RMSNorm 82 -> 75 / 76 -> 70 us, with the residual
+  // 129 -> 121 / 124 -> 118; asked for before the residual's loads they gain nothing there.
   if constexpr (norm_rows(MODE)) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
